@@ -381,6 +381,124 @@ int moe_regroup_gather(moe_sampler* sampler, void* stream, const float* hidden, 
  * reference indexes its host vector unchecked. */
 int moe_regroup_gather_check(moe_sampler* sampler, void* stream, int32_t* out_of_range);
 
+/* ---- expert products ------------------------------------------------------ */
+
+/* What follows the dispatch on the device: the experts' matrix products on the
+ * regrouped rows, in 8-bit floating point with a scale for each block of 128,
+ * and their way back to the tokens.  The reference runs its experts on the host
+ * or through ncnn (src/kernels, ExpertDispatchPlan consumers); these calls take
+ * the plan of moe_router_dispatch as it lies on the device.
+ *
+ * e4m3 values are the OCP format without infinities (largest 448, NaN 0x7F). */
+#define MOE_EXPERT_BLOCK 128u        /* columns that share a scale */
+#define MOE_EXPERT_MAX_EXPERTS 4096u /* largest expert_count of these calls, as for the router */
+
+enum moe_activation
+{
+    MOE_ACTIVATION_NONE = 0,
+    MOE_ACTIVATION_SILU_GATE = 1 /* x = gate / (1 + exp(-gate)) * up, gate and up being the two halves of a source row */
+};
+
+/* Rows to e4m3 with one fp32 scale per block of 128 columns (the last block of a
+ * row may be shorter):
+ *   scale = max |x| / 448,  value = e4m3(x / scale), to nearest, ties to even
+ * with the quotients rounded to fp32; a block of zeros has scale 0 and values 0.
+ * NaN gives NaN; an infinity makes its whole block decode to NaN.
+ *
+ * source       device, [source_rows x row_stride] of dtype (moe_dtype); columns entries of a
+ *              row are used, 2 * columns with MOE_ACTIVATION_SILU_GATE
+ * route_token  device, route_count entries, or NULL.  With it, output row i is source row
+ *              route_token[i] (the regroup gather in the same pass); without it, output row i
+ *              is source row i and route_count is ignored.  An entry >= source_rows is never
+ *              dereferenced: its row has scales and values 0 and the handle remembers
+ *              MOE_EXPERT_FLAG_TOKEN_RANGE.
+ * values       device, [rows x columns] e4m3, dense
+ * scales       device, [ceil(columns / 128) x rows]: block-major
+ * Asynchronous on `stream`; allocates nothing. */
+int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,
+                      int activation, const uint32_t* route_token, uint32_t route_count, uint8_t* values, float* scales);
+
+/* Each expert's rows times its weights, transposed:
+ *   out[r, n] = sum over blocks b of scales[b, r] * weight_scales[e, n / 128, b] * sum over k in b of values[r, k] * weights[e, n, k]
+ * e being the expert whose range [expert_offsets[e], expert_offsets[e + 1]) holds r.  Sums are fp32.
+ *
+ * values, scales   device, as moe_quantize_rows writes them: [rows x columns], [ceil(columns / 128) x rows]
+ * weights          device, [expert_count x outputs x columns] e4m3, dense
+ * weight_scales    device, [expert_count x ceil(outputs / 128) x ceil(columns / 128)]
+ * expert_offsets   device, expert_count + 1 ascending entries (those of a dispatch plan), or NULL
+ *                  with expert_count 1: all rows are that expert's (a dense product)
+ * out              device, [rows x out_stride] of out_dtype (moe_dtype), outputs <= out_stride entries written per row
+ * Rows outside every expert's range are left as they were.  Offsets that descend or exceed `rows` are
+ * not followed: nothing is written and the handle remembers MOE_EXPERT_FLAG_OFFSETS.
+ * columns must be a multiple of 16, values and weights 16-byte aligned; expert_count <= MOE_EXPERT_MAX_EXPERTS;
+ * rows, outputs, columns and expert_count * outputs < 2^31.
+ * Asynchronous on `stream`; allocates nothing. */
+int moe_expert_product(moe_sampler* sampler, void* stream, const uint8_t* values, const float* scales, uint32_t rows, uint32_t columns,
+                       const uint8_t* weights, const float* weight_scales, uint32_t expert_count, uint32_t outputs, const uint32_t* expert_offsets,
+                       void* out, int out_dtype, size_t out_stride);
+
+/* The routed rows back to their tokens (the Combine step behind the experts of
+ * src/engine/cpu_executor.cpp):
+ *   out[t, :] = base[t, :] + sum over the routes of t, ranks ascending, of route_weight * route_rows[route, :]
+ * in fp32, rounded once.
+ *
+ * route_rows   device, [route_count x row_stride] of dtype, columns <= row_stride used
+ * route_token, route_rank, route_weight  device, route_count entries of a dispatch plan.  A route whose token is
+ *              >= token_count or whose rank is >= top_k is left out and the handle remembers
+ *              MOE_EXPERT_FLAG_TOKEN_RANGE; of several routes with the same token and rank the last counts.
+ * base         device, [token_count x columns] of dtype, or NULL; may be `out`
+ * out          device, [token_count x columns] of dtype; a token without routes gets its base, or zeros
+ * Asynchronous on `stream`.  Calls with more routes than any before on this handle grow its scratch
+ * (token_count * top_k words); make the largest one before a stream capture. */
+int moe_combine_routes(moe_sampler* sampler, void* stream, const void* route_rows, int dtype, size_t row_stride, uint32_t columns,
+                       const uint32_t* route_token, const uint32_t* route_rank, const float* route_weight, uint32_t route_count, uint32_t token_count,
+                       uint32_t top_k, const void* base, void* out);
+
+/* Bits that moe_expert_check reports. */
+#define MOE_EXPERT_FLAG_TOKEN_RANGE 1u /* a route named a token (or rank) outside the call */
+#define MOE_EXPERT_FLAG_OFFSETS 2u     /* expert_offsets descended or exceeded the rows */
+#define MOE_EXPERT_FLAG_STALLED 4u     /* a wait inside moe_expert_product ran out: its output is incomplete */
+
+/* Synchronises `stream`, stores the MOE_EXPERT_FLAG_* bits that calls on this handle have met since the
+ * last check in *flags, and clears them. */
+int moe_expert_check(moe_sampler* sampler, void* stream, uint32_t* flags);
+
+/* ---- expert balance ------------------------------------------------------- */
+
+/* How evenly a batch uses its experts, and the balance loss that trains the router towards it.  With p the
+ * scores of a token divided by their sum over the experts (softmax rows already sum to 1), n the tokens
+ * that count, c_e the routes of those tokens that went to expert e, E experts and k routes a token:
+ *   P_e = sum of p_e over the tokens / n,   loss = coefficient * sum over e of (E * c_e / (k * n)) * P_e
+ * A token whose scores are all zero counts, with p = 0.  With n = 0 all results are 0.  Non-finite logits
+ * (which moe_router_dispatch refuses) give what the arithmetic gives.
+ *
+ * router_logits   device, [token_count x expert_count], as for moe_router_dispatch
+ * options         expert_count, top_k and score_function are used (host)
+ * expert_offsets, route_token   device, of the plan that moe_router_dispatch made from the same logits.  Offsets
+ *                 that descend or exceed token_count * top_k are not followed (no route counts,
+ *                 MOE_EXPERT_FLAG_OFFSETS); a route_token entry >= token_count is not counted
+ *                 (MOE_EXPERT_FLAG_TOKEN_RANGE).
+ * token_mask      device, token_count bytes, or NULL: tokens with a 0 (padding) do not count
+ * expert_tokens   device, [expert_count + 1]: c_e, then n
+ * expert_probability  device, [expert_count]: P_e
+ * loss            device, one float
+ * Sums have a fixed order: equal inputs give equal bits.  Asynchronous on `stream`; the first call on a handle, and
+ * one with more experts than any before, allocates scratch: make it before a stream capture. */
+int moe_balance_loss(moe_sampler* sampler, void* stream, const float* router_logits, uint32_t token_count, const moe_router_options* options,
+                     const uint32_t* expert_offsets, const uint32_t* route_token, const uint8_t* token_mask, float coefficient, uint32_t* expert_tokens,
+                     float* expert_probability, float* loss);
+
+/* The gradient of that loss with respect to the router logits (the counts c_e are constants, as usual):
+ *   logit_gradient[t, e] = loss_gradient * dloss / dlogit[t, e], zeros for tokens that do not count
+ *
+ * expert_tokens   device, [expert_count + 1] as moe_balance_loss wrote it
+ * loss_gradient   device, one float, or NULL for 1
+ * logit_gradient  device, [token_count x expert_count]; overwritten
+ * The other arguments are those of the forward call.  Asynchronous on `stream`; allocates nothing. */
+int moe_balance_loss_backward(moe_sampler* sampler, void* stream, const float* router_logits, uint32_t token_count, const moe_router_options* options,
+                              const uint8_t* token_mask, float coefficient, const uint32_t* expert_tokens, const float* loss_gradient,
+                              float* logit_gradient);
+
 /* ---- latent-attention indexer ------------------------------------------- */
 
 /* Replaces the selection at the end of select_compressed_indices

@@ -24,6 +24,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",
     "-shared",
+    "--threads", "0",  # the sources side by side
 ]
 
 

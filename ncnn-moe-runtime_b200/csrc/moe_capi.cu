@@ -72,6 +72,14 @@ struct moe_sampler
     uint32_t* router_scan_done = nullptr;    // one word, 0 between calls
     uint32_t* router_block_counts = nullptr; // [MOE_ROUTER_BLOCK_TABLE_ENTRIES], allocated by the first router call
     int32_t* gather_status = nullptr;        // one word: set when moe_regroup_gather met a token index out of range
+    // expert products and balance
+    uint32_t* expert_flags = nullptr;  // one word: MOE_EXPERT_FLAG_* met since the last check
+    uint32_t* combine_slots = nullptr; // zeros between calls
+    size_t combine_slots_capacity = 0;
+    float* balance_sums = nullptr;
+    uint32_t* balance_counts = nullptr;
+    size_t balance_sums_capacity = 0;
+    size_t balance_counts_capacity = 0;
     // router host staging
     float* router_logits_dev = nullptr;
     size_t router_logits_capacity = 0;
@@ -301,6 +309,7 @@ int moe_sampler_create(int device, uint32_t max_rows, uint32_t max_vocab, moe_sa
     allocate(reinterpret_cast<void**>(&sampler->router_scan_done), sizeof(uint32_t));
     allocate(reinterpret_cast<void**>(&sampler->gather_status), sizeof(int32_t));
     allocate(reinterpret_cast<void**>(&sampler->router_status_dev), sizeof(int32_t));
+    allocate(reinterpret_cast<void**>(&sampler->expert_flags), sizeof(uint32_t));
     if (status == cudaSuccess)
         status = cudaMemset(counters, 0, 8 * sizeof(uint32_t));
     if (status == cudaSuccess)
@@ -311,6 +320,8 @@ int moe_sampler_create(int device, uint32_t max_rows, uint32_t max_vocab, moe_sa
         status = cudaMemset(sampler->router_scan_done, 0, sizeof(uint32_t));
     if (status == cudaSuccess)
         status = cudaMemset(sampler->gather_status, 0, sizeof(int32_t));
+    if (status == cudaSuccess)
+        status = cudaMemset(sampler->expert_flags, 0, sizeof(uint32_t));
     if (status == cudaSuccess)
         status = cudaStreamCreateWithFlags(&sampler->stream, cudaStreamNonBlocking);
     if (status == cudaSuccess)
@@ -344,7 +355,8 @@ void moe_sampler_destroy(moe_sampler* sampler)
                         sampler->router_offsets_dev, sampler->router_token_dev, sampler->router_rank_dev, sampler->router_weight_dev,
                         sampler->router_status_dev, sampler->spec_kept_token, sampler->spec_kept_probability, sampler->spec_kept_count,
                         sampler->spec_token, sampler->spec_probability, sampler->spec_flags, sampler->spec_status, sampler->spec_dense,
-                        sampler->spec_residual_token, sampler->spec_residual_value};
+                        sampler->spec_residual_token, sampler->spec_residual_value, sampler->expert_flags, sampler->combine_slots,
+                        sampler->balance_sums, sampler->balance_counts};
     for (void* pointer : pointers)
         if (pointer != nullptr)
             cudaFree(pointer);
@@ -1036,6 +1048,133 @@ int moe_regroup_gather_check(moe_sampler* sampler, void* stream_handle, int32_t*
     MOE_CUDA_CHECK(sampler, cudaMemcpyAsync(out_of_range, sampler->gather_status, sizeof(int32_t), cudaMemcpyDeviceToHost, stream));
     MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->gather_status, 0, sizeof(int32_t), stream));
     MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
+    return MOE_STATUS_OK;
+}
+
+int moe_quantize_rows(moe_sampler* sampler, void* stream_handle, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,
+                      int activation, const uint32_t* route_token, uint32_t route_count, uint8_t* values, float* scales)
+{
+    if (sampler == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    const QuantizeArgs args = {source, source_rows, route_token != nullptr ? route_count : source_rows, columns, row_stride, route_token, values, scales, sampler->expert_flags};
+    if (const char* text = check_quantize(args, dtype, activation))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
+    if (args.rows == 0 || columns == 0)
+        return MOE_STATUS_OK;
+    DeviceGuard guard(sampler->device);
+    MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, static_cast<cudaStream_t>(stream_handle)));
+    return MOE_STATUS_OK;
+}
+
+int moe_expert_product(moe_sampler* sampler, void* stream_handle, const uint8_t* values, const float* scales, uint32_t rows, uint32_t columns,
+                       const uint8_t* weights, const float* weight_scales, uint32_t expert_count, uint32_t outputs, const uint32_t* expert_offsets,
+                       void* out, int out_dtype, size_t out_stride)
+{
+    if (sampler == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    const ProductArgs args = {values, scales, rows, columns, weights, weight_scales, expert_count, outputs, expert_offsets, out, out_stride, sampler->expert_flags};
+    if (const char* text = check_product(args, out_dtype))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
+    if (rows == 0)
+        return MOE_STATUS_OK;
+    DeviceGuard guard(sampler->device);
+    MOE_CUDA_CHECK(sampler, launch_expert_product(args, out_dtype, static_cast<cudaStream_t>(stream_handle)));
+    return MOE_STATUS_OK;
+}
+
+int moe_combine_routes(moe_sampler* sampler, void* stream_handle, const void* route_rows, int dtype, size_t row_stride, uint32_t columns,
+                       const uint32_t* route_token, const uint32_t* route_rank, const float* route_weight, uint32_t route_count, uint32_t token_count,
+                       uint32_t top_k, const void* base, void* out)
+{
+    if (sampler == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    CombineArgs args = {route_rows, row_stride, columns, route_token, route_rank, route_weight, route_count, token_count, top_k, base, out, nullptr, sampler->expert_flags};
+    if (const char* text = check_combine(args, dtype))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
+    if (token_count == 0 || columns == 0)
+        return MOE_STATUS_OK;
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+    DeviceGuard guard(sampler->device);
+    const size_t slots = static_cast<size_t>(token_count) * top_k;
+    if (slots > sampler->combine_slots_capacity)
+    {
+        // earlier calls on this stream may still use the scratch that is replaced here
+        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
+        MOE_CUDA_CHECK(sampler, grow(sampler->combine_slots, sampler->combine_slots_capacity, slots));
+        MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->combine_slots, 0, sizeof(uint32_t) * slots, stream));
+    }
+    args.slots = sampler->combine_slots;
+    MOE_CUDA_CHECK(sampler, launch_combine_routes(args, dtype, stream));
+    return MOE_STATUS_OK;
+}
+
+int moe_expert_check(moe_sampler* sampler, void* stream_handle, uint32_t* flags)
+{
+    if (sampler == nullptr || flags == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    DeviceGuard guard(sampler->device);
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+    MOE_CUDA_CHECK(sampler, cudaMemcpyAsync(flags, sampler->expert_flags, sizeof(uint32_t), cudaMemcpyDeviceToHost, stream));
+    MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->expert_flags, 0, sizeof(uint32_t), stream));
+    MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
+    return MOE_STATUS_OK;
+}
+
+int moe_balance_loss(moe_sampler* sampler, void* stream_handle, const float* router_logits, uint32_t token_count, const moe_router_options* options,
+                     const uint32_t* expert_offsets, const uint32_t* route_token, const uint8_t* token_mask, float coefficient, uint32_t* expert_tokens,
+                     float* expert_probability, float* loss)
+{
+    if (sampler == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    const int precheck = moe_router_check_options(token_count, options);
+    if (precheck != 0)
+        return fail(sampler, moe_router_status_error_code(precheck), moe_router_status_message(precheck));
+    BalanceArgs args = {router_logits, token_count, options->expert_count, options->top_k, options->score_function, coefficient, token_mask,
+                        expert_offsets, route_token, expert_tokens, expert_probability, loss, nullptr, nullptr, sampler->expert_flags};
+    if (const char* text = check_balance(args))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
+    if (router_logits == nullptr || expert_offsets == nullptr || route_token == nullptr || expert_tokens == nullptr || expert_probability == nullptr ||
+        loss == nullptr)
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, "balance buffers must not be null");
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+    DeviceGuard guard(sampler->device);
+    const size_t sums = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * options->expert_count;
+    const size_t counts = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * (options->expert_count + 1u);
+    if (sums > sampler->balance_sums_capacity || counts > sampler->balance_counts_capacity)
+    {
+        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
+        MOE_CUDA_CHECK(sampler, grow(sampler->balance_sums, sampler->balance_sums_capacity, sums));
+        MOE_CUDA_CHECK(sampler, grow(sampler->balance_counts, sampler->balance_counts_capacity, counts));
+    }
+    args.partial_sums = sampler->balance_sums;
+    args.partial_counts = sampler->balance_counts;
+    MOE_CUDA_CHECK(sampler, launch_balance_loss(args, stream));
+    return MOE_STATUS_OK;
+}
+
+int moe_balance_loss_backward(moe_sampler* sampler, void* stream_handle, const float* router_logits, uint32_t token_count, const moe_router_options* options,
+                              const uint8_t* token_mask, float coefficient, const uint32_t* expert_tokens, const float* loss_gradient,
+                              float* logit_gradient)
+{
+    if (sampler == nullptr)
+        return MOE_STATUS_INVALID_ARGUMENT;
+    const int precheck = moe_router_check_options(token_count, options);
+    if (precheck != 0)
+        return fail(sampler, moe_router_status_error_code(precheck), moe_router_status_message(precheck));
+    BalanceArgs args = {};
+    args.logits = router_logits;
+    args.token_count = token_count;
+    args.expert_count = options->expert_count;
+    args.top_k = options->top_k;
+    args.score_function = options->score_function;
+    args.coefficient = coefficient;
+    args.token_mask = token_mask;
+    if (const char* text = check_balance(args))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
+    if (router_logits == nullptr || expert_tokens == nullptr || logit_gradient == nullptr)
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, "balance buffers must not be null");
+    DeviceGuard guard(sampler->device);
+    MOE_CUDA_CHECK(sampler, launch_balance_loss_backward(args, expert_tokens, loss_gradient, logit_gradient, static_cast<cudaStream_t>(stream_handle)));
     return MOE_STATUS_OK;
 }
 

@@ -17,6 +17,8 @@
 #define MOE_SPECULATIVE_SHORT_LIST 1024u
 // entries of the router's [expert][block] count table (expert_count * blocks of the select kernel never exceeds it)
 #define MOE_ROUTER_BLOCK_TABLE_ENTRIES 262144u
+// blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): two per SM
+#define MOE_BALANCE_MAX_BLOCKS 296u
 
 namespace moe {
 
@@ -298,6 +300,163 @@ cudaError_t launch_following(void (*kernel)(Parameters...), uint32_t grid, uint3
 // order, 0xFFFFFFFF beyond min(top_k, count); out_score may be null.  top_k <= MOE_INDEXER_TOPK_MAX.
 cudaError_t launch_indexer_topk(const float* scores, uint32_t rows, uint32_t count, size_t row_stride, uint32_t top_k, uint32_t* out_index,
                                 float* out_score, int sm_count, cudaStream_t stream);
+
+// ---- expert products and balance ----
+
+struct QuantizeArgs
+{
+    const void* source;
+    uint32_t source_rows;
+    uint32_t rows; // output rows
+    uint32_t columns;
+    size_t row_stride;
+    const uint32_t* route_token; // [rows] or null
+    uint8_t* values;
+    float* scales;
+    uint32_t* flags; // MOE_EXPERT_FLAG_* of the handle
+};
+struct ProductArgs
+{
+    const uint8_t* values;
+    const float* scales;
+    uint32_t rows;
+    uint32_t columns;
+    const uint8_t* weights;
+    const float* weight_scales;
+    uint32_t expert_count;
+    uint32_t outputs;
+    const uint32_t* expert_offsets; // null: all rows are expert 0's
+    void* out;
+    size_t out_stride;
+    uint32_t* flags;
+};
+struct CombineArgs
+{
+    const void* route_rows;
+    size_t row_stride;
+    uint32_t columns;
+    const uint32_t* route_token;
+    const uint32_t* route_rank;
+    const float* route_weight;
+    uint32_t route_count;
+    uint32_t token_count;
+    uint32_t top_k;
+    const void* base; // may be null
+    void* out;
+    uint32_t* slots; // [token_count * top_k], 0 between calls: route + 1 of every (token, rank)
+    uint32_t* flags;
+};
+struct BalanceArgs
+{
+    const float* logits;
+    uint32_t token_count;
+    uint32_t expert_count;
+    uint32_t top_k;
+    int score_function;
+    float coefficient;
+    const uint8_t* token_mask; // may be null
+    // forward only
+    const uint32_t* expert_offsets;
+    const uint32_t* route_token;
+    uint32_t* expert_tokens;
+    float* expert_probability;
+    float* loss;
+    float* partial_sums;      // [MOE_BALANCE_MAX_BLOCKS][expert_count]
+    uint32_t* partial_counts; // [MOE_BALANCE_MAX_BLOCKS][expert_count + 1]
+    uint32_t* flags;
+};
+cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, cudaStream_t stream);
+cudaError_t launch_expert_product(const ProductArgs& args, int out_dtype, cudaStream_t stream);
+cudaError_t launch_combine_routes(const CombineArgs& args, int dtype, cudaStream_t stream);
+cudaError_t launch_balance_loss(const BalanceArgs& args, cudaStream_t stream);
+cudaError_t launch_balance_loss_backward(const BalanceArgs& args, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient, cudaStream_t stream);
+
+// The checks of these calls that need no data: the text of the first one that fails, or null.
+inline const char* check_value_type(int dtype)
+{
+    return dtype == MOE_DTYPE_F32 || dtype == MOE_DTYPE_BF16 ? nullptr : "dtype must be MOE_DTYPE_F32 or MOE_DTYPE_BF16";
+}
+inline bool misaligned(const void* pointer, size_t bytes)
+{
+    return reinterpret_cast<uintptr_t>(pointer) % bytes != 0u;
+}
+// value arrays of a caller's type start at a multiple of their element
+inline bool misaligned_values(const void* pointer, int dtype)
+{
+    return misaligned(pointer, dtype == MOE_DTYPE_F32 ? 4u : 2u);
+}
+inline const char* check_quantize(const QuantizeArgs& a, int dtype, int activation)
+{
+    if (const char* text = check_value_type(dtype))
+        return text;
+    if (activation != MOE_ACTIVATION_NONE && activation != MOE_ACTIVATION_SILU_GATE)
+        return "activation must be MOE_ACTIVATION_NONE or MOE_ACTIVATION_SILU_GATE";
+    const size_t used = static_cast<size_t>(a.columns) * (activation == MOE_ACTIVATION_SILU_GATE ? 2u : 1u);
+    if (a.row_stride < used)
+        return "row_stride is smaller than the columns a row uses";
+    if (a.columns > 0x7FFFFFFFu)
+        return "columns must be below 2^31";
+    if (a.rows == 0 || a.columns == 0)
+        return nullptr;
+    if ((a.source == nullptr && a.source_rows > 0) || a.values == nullptr || a.scales == nullptr)
+        return "source, values and scales must not be null";
+    if (misaligned_values(a.source, dtype) || misaligned(a.scales, 4u) || misaligned(a.route_token, 4u))
+        return "source, scales and route_token must be aligned to their elements";
+    return nullptr;
+}
+inline const char* check_product(const ProductArgs& a, int out_dtype)
+{
+    if (check_value_type(out_dtype) != nullptr)
+        return "out_dtype must be MOE_DTYPE_F32 or MOE_DTYPE_BF16";
+    if (a.expert_count == 0 || a.expert_count > MOE_EXPERT_MAX_EXPERTS)
+        return "expert products need 0 < expert_count <= MOE_EXPERT_MAX_EXPERTS";
+    if (a.expert_offsets == nullptr && a.expert_count != 1)
+        return "expert_offsets may only be null with one expert";
+    if (a.columns == 0 || a.columns % 16u != 0)
+        return "expert products need columns to be a positive multiple of 16";
+    if (a.outputs == 0 || a.columns > 0x7FFFFFFFu || a.rows > 0x7FFFFFFFu || static_cast<uint64_t>(a.expert_count) * a.outputs > 0x7FFFFFFFull)
+        return "expert products need outputs > 0 and rows, columns and expert_count * outputs below 2^31";
+    if (a.out_stride < a.outputs)
+        return "out_stride is smaller than outputs";
+    if (a.rows == 0)
+        return nullptr;
+    if (a.values == nullptr || a.scales == nullptr || a.weights == nullptr || a.weight_scales == nullptr || a.out == nullptr)
+        return "values, scales, weights, weight_scales and out must not be null";
+    if (misaligned(a.values, 16u) || misaligned(a.weights, 16u))
+        return "values and weights must be 16-byte aligned";
+    if (misaligned(a.scales, 4u) || misaligned(a.weight_scales, 4u) || misaligned(a.expert_offsets, 4u) || misaligned_values(a.out, out_dtype))
+        return "scales, weight_scales, expert_offsets and out must be aligned to their elements";
+    return nullptr;
+}
+inline const char* check_combine(const CombineArgs& a, int dtype)
+{
+    if (const char* text = check_value_type(dtype))
+        return text;
+    if (a.row_stride < a.columns)
+        return "row_stride is smaller than columns";
+    if (a.columns > 0x7FFFFFFFu || a.token_count > 0x7FFFFFFFu || a.route_count > 0x7FFFFFFFu)
+        return "columns, token_count and route_count must be below 2^31";
+    if (a.token_count == 0 || a.columns == 0)
+        return nullptr;
+    if (a.top_k == 0 && a.route_count > 0)
+        return "top_k must be positive";
+    if (a.out == nullptr)
+        return "out must not be null";
+    if (a.route_count > 0 && (a.route_rows == nullptr || a.route_token == nullptr || a.route_rank == nullptr || a.route_weight == nullptr))
+        return "route_rows, route_token, route_rank and route_weight must not be null";
+    if (misaligned_values(a.route_rows, dtype) || misaligned_values(a.base, dtype) || misaligned_values(a.out, dtype) || misaligned(a.route_token, 4u) ||
+        misaligned(a.route_rank, 4u) || misaligned(a.route_weight, 4u))
+        return "combine buffers must be aligned to their elements";
+    return nullptr;
+}
+inline const char* check_balance(const BalanceArgs& a)
+{
+    if (a.score_function != MOE_ROUTER_SOFTMAX && a.score_function != MOE_ROUTER_SIGMOID && a.score_function != MOE_ROUTER_SQRT_SOFTPLUS)
+        return "score_function must be a moe_router_score";
+    if (!(a.coefficient - a.coefficient == 0.0f))
+        return "the balance coefficient must be finite";
+    return nullptr;
+}
 
 uint32_t choose_splits(uint32_t rows, uint32_t vocab, int dtype, int sm_count, uint32_t slice_slots, bool large_top_k, bool overlapped);
 
