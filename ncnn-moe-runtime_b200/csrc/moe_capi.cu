@@ -1078,7 +1078,7 @@ int moe_expert_product(moe_sampler* sampler, void* stream_handle, const uint8_t*
     if (rows == 0)
         return MOE_STATUS_OK;
     DeviceGuard guard(sampler->device);
-    MOE_CUDA_CHECK(sampler, launch_expert_product(args, out_dtype, static_cast<cudaStream_t>(stream_handle)));
+    MOE_CUDA_CHECK(sampler, launch_expert_product(args, out_dtype, sampler->sm_count, static_cast<cudaStream_t>(stream_handle)));
     return MOE_STATUS_OK;
 }
 

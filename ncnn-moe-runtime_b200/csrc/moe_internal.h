@@ -366,7 +366,7 @@ struct BalanceArgs
     uint32_t* flags;
 };
 cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, cudaStream_t stream);
-cudaError_t launch_expert_product(const ProductArgs& args, int out_dtype, cudaStream_t stream);
+cudaError_t launch_expert_product(const ProductArgs& args, int out_dtype, int sm_count, cudaStream_t stream);
 cudaError_t launch_combine_routes(const CombineArgs& args, int dtype, cudaStream_t stream);
 cudaError_t launch_balance_loss(const BalanceArgs& args, cudaStream_t stream);
 cudaError_t launch_balance_loss_backward(const BalanceArgs& args, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient, cudaStream_t stream);
