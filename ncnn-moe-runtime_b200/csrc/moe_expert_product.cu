@@ -37,9 +37,9 @@ struct Shape
     static constexpr uint32_t kStages = kTokens <= 16 ? 10u : kTokens <= 32 ? 9u : kTokens <= 64 ? 8u : kTokens <= 128 ? 6u : 4u;
     static constexpr uint32_t kAccumulators = kTokens <= 128 ? 4u : 2u;
     static constexpr uint32_t kMemoryColumns = kTokens * kAccumulators < 32 ? 32u : kTokens * kAccumulators;
-    static constexpr uint32_t kSumWarps = kTokens <= 128 ? 4u : 8u;
+    static constexpr uint32_t kSumWarps = kTokens <= 64 ? 4u : 8u;
     static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
-    static constexpr uint32_t kColumns = kTokens <= 128 ? kTokens : 128u; // columns of the tile that a warp sums
+    static constexpr uint32_t kColumns = kTokens / (kSumWarps / 4u);      // columns of the tile that a warp sums
     static constexpr uint32_t kChunk = kColumns < 32u ? kColumns : 32u;   // columns read from tensor memory at once
     static constexpr uint32_t kScaleBytes = kScaleSlots * kTokens * 4u;
     static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators + 2u * kScaleSlots;
@@ -171,6 +171,21 @@ __device__ __forceinline__ void add_scaled_pair(uint64_t& sum, uint32_t part_low
         "}\n"
         : "+l"(sum)
         : "r"(part_low), "r"(part_high), "l"(factors));
+}
+
+// One thread of a whole warp.  Not a comparison of the lane: behind that the compiler feeds every instruction of the tensor
+// cores and the copy engine through code for several lanes (a block of 128 columns took about 1000 cycles to issue).
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t elected;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xFFFFFFFF;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(elected));
+    return elected != 0u;
 }
 
 // ---- tiles ------------------------------------------------------------------------------
@@ -336,7 +351,7 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
 
     if (warp == 0u)
     {
-        if (lane == 0u)
+        if (elect_one())
         {
             Cursor cursor;
             uint32_t issued = 0;
@@ -369,7 +384,7 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
     }
     else if (warp == 1u)
     {
-        if (lane == 0u)
+        if (elect_one())
         {
             Cursor cursor, sum;
             bool running = true;
@@ -486,18 +501,23 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t factors = scale_slots + (scale.slot * kTokens + first_column) * 4u;
                 const uint32_t source = memory + sum.slot * kTokens;
+                // the next chunk is on its way while this one is summed
+                constexpr uint32_t kChunks = S::kColumns / S::kChunk;
+                uint32_t part[2][S::kChunk];
+                load_accumulator<S::kChunk>(part[0], source);
 #pragma unroll
-                for (uint32_t chunk = 0; chunk < S::kColumns / S::kChunk; ++chunk)
+                for (uint32_t chunk = 0; chunk < kChunks; ++chunk)
                 {
-                    uint32_t part[S::kChunk];
-                    load_accumulator<S::kChunk>(part, source + chunk * S::kChunk);
-                    wait_accumulator<S::kChunk>(part);
+                    wait_accumulator<S::kChunk>(part[chunk & 1u]);
+                    if (chunk + 1u < kChunks)
+                        load_accumulator<S::kChunk>(part[(chunk + 1u) & 1u], source + (chunk + 1u) * S::kChunk);
 #pragma unroll
                     for (uint32_t i = 0; i < S::kChunk; i += 4u)
                     {
                         const ulonglong2 factor = load_shared_2x64(factors + (chunk * S::kChunk + i) * 4u);
-                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u], part[i], part[i + 1u], factor.x);
-                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u + 1u], part[i + 2u], part[i + 3u], factor.y);
+                        const uint32_t(&p)[S::kChunk] = part[chunk & 1u];
+                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u], p[i], p[i + 1u], factor.x);
+                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u + 1u], p[i + 2u], p[i + 3u], factor.y);
                     }
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
