@@ -1,192 +1,29 @@
 // The experts' matrix products in e4m3 with a scale for each block of 128:
 //   out[r, n] = sum_b scales[b, r] * weight_scales[e, n / 128, b] * sum_{k in b} values[r, k] * weights[e, n, k]
 //
-// The weights are the tall operand: a tile is 128 outputs (the 128 lanes of the accumulator in tensor memory) by kTokens
-// rows (its columns), so that a few rows of a decode step do not fill a tile of 128 rows with padding, and a tile's outputs
-// lie in one block of the weights' scales.  Per block of 128 columns the tensor cores compute the inner sum into a fresh
-// accumulator, four instructions of 32 columns each, and the epilogue warps add it to their registers times the product of
-// the two scales: one fused multiply-add per element of the tile and block, with a factor that all 128 lanes share per
-// column.
-//
-// Roles of a CTA, which stays for all its tiles: a thread that requests tiles of both operands from the copy engine, a
-// thread that issues the products, a warp that multiplies the scales, four or eight warps that scale, sum and store.  They
-// pass a ring of operand stages, two to four accumulators and a ring of scales to each other through mbarriers, so that the
-// copies, the products and the sums of different blocks, and of different tiles, overlap.
+// Per block of 128 columns the tensor cores compute the inner sums of a tile into a fresh accumulator in tensor memory, four
+// instructions of 32 columns each; other warps read it out and add it to their registers times the product of the two scales,
+// one fused multiply-add per element of the tile and block.  Two kernels:
+//   few rows an expert   a tile is 128 outputs (the 128 lanes of an accumulator) by 16, 32 or 64 rows (its columns): the rows of
+//                        a decode step do not fill a tile of 128 with padding.  Bound by the weights from HBM.
+//   many rows            a tile is 128 rows by 256 outputs, or 256 by 256 on a pair of SMs: a thread sums for one row, so that a
+//                        block's factor is one register.  Bound by the tensor cores, by L2 or by the weights.
+// Roles of a CTA, which stays for all its tiles: a thread that requests tiles of both operands from the copy engine, threads
+// that issue the products, warps that scale, sum and store.  They pass a ring of operand stages and a few accumulators to each
+// other through mbarriers, so that copies, products and sums of different blocks, and of different tiles, overlap.
 
-#include <cuda.h>
-
-#include "moe_common.cuh"
 #include "moe_internal.h"
+#include "moe_tensor.cuh"
 
 namespace moe {
 
 namespace {
 
-constexpr uint32_t kOutputs = 128;      // outputs of a tile
 constexpr uint32_t kBlockBytes = MOE_EXPERT_BLOCK;
-constexpr uint32_t kWeightTile = kOutputs * kBlockBytes;
-constexpr uint32_t kScaleSlots = 8;     // blocks of scales in flight
+constexpr uint32_t kLanes = 128;        // of an accumulator
+constexpr uint32_t kTallTile = kLanes * kBlockBytes;
 constexpr uint32_t kGroupTiles = 16;    // row tiles that share a weight tile before the next one is taken
-constexpr uint32_t kSpinLimit = 1u << 20;
-constexpr uint32_t kRoleThreads = 128;  // one warp for the copies, one for the products, one for the scales, one for tensor memory
-
-template<int kTokens>
-struct Shape
-{
-    static constexpr uint32_t kStageBytes = kWeightTile + kTokens * kBlockBytes;
-    static constexpr uint32_t kStages = kTokens <= 16 ? 10u : kTokens <= 32 ? 9u : kTokens <= 64 ? 8u : kTokens <= 128 ? 6u : 4u;
-    static constexpr uint32_t kAccumulators = kTokens <= 128 ? 4u : 2u;
-    static constexpr uint32_t kMemoryColumns = kTokens * kAccumulators < 32 ? 32u : kTokens * kAccumulators;
-    static constexpr uint32_t kSumWarps = kTokens <= 64 ? 4u : 8u;
-    static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
-    static constexpr uint32_t kColumns = kTokens / (kSumWarps / 4u);      // columns of the tile that a warp sums
-    static constexpr uint32_t kChunk = kColumns < 32u ? kColumns : 32u;   // columns read from tensor memory at once
-    static constexpr uint32_t kScaleBytes = kScaleSlots * kTokens * 4u;
-    static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators + 2u * kScaleSlots;
-    static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kScaleBytes + kBarriers * 8u + 64u;
-};
-
-// ---- mbarriers, tensor memory, descriptors ---------------------------------------------
-
-__device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t arrivals)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(arrivals) : "memory");
-}
-__device__ __forceinline__ void barrier_arrive(uint32_t barrier)
-{
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
-}
-__device__ __forceinline__ void barrier_expect_bytes(uint32_t barrier, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool barrier_test(uint32_t barrier, uint32_t parity)
-{
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(barrier), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-// Bounded.  A wait that runs out marks the CTA as stalled; every role then leaves its loop.
-__device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, volatile uint32_t* stalled)
-{
-    for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
-    {
-        if (barrier_test(barrier, parity))
-            return true;
-        if ((spin & 255u) == 255u && *stalled != 0u)
-            return false;
-    }
-    *stalled = 1u;
-    return false;
-}
-
-__device__ __forceinline__ void copy_tile(uint32_t destination, const CUtensorMap* map, uint32_t column, uint32_t row, uint32_t barrier)
-{
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(destination), "l"(map),
-                 "r"(column), "r"(row), "r"(barrier)
-                 : "memory");
-}
-// A tile in shared memory as the copy engine leaves it: rows of 128 bytes, swizzled in groups of eight rows (1024 bytes
-// from group to group).  A step of 32 columns moves the start by 32 bytes.
-__device__ __forceinline__ uint64_t tile_descriptor(uint32_t address)
-{
-    return static_cast<uint64_t>((address & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-// e4m3 by e4m3 into fp32, both operands with adjacent columns, 128 x kTokens
-template<int kTokens>
-__device__ __forceinline__ constexpr uint32_t product_descriptor()
-{
-    return (1u << 4) | (static_cast<uint32_t>(kTokens >> 3) << 17) | ((kOutputs >> 4) << 24);
-}
-__device__ __forceinline__ void issue_product(uint32_t accumulator, uint64_t weights, uint64_t rows, uint32_t descriptor, bool accumulate)
-{
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(accumulator),
-        "l"(weights), "l"(rows), "r"(descriptor), "r"(accumulate ? 1u : 0u)
-        : "memory");
-}
-// arrives at the barrier once the products issued so far are done
-__device__ __forceinline__ void commit_products(uint32_t barrier)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
-}
-
-template<int kCount>
-__device__ __forceinline__ void load_accumulator(uint32_t (&t)[kCount], uint32_t address);
-template<>
-__device__ __forceinline__ void load_accumulator<16>(uint32_t (&t)[16], uint32_t address)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]), "=r"(t[4]), "=r"(t[5]), "=r"(t[6]), "=r"(t[7]), "=r"(t[8]), "=r"(t[9]), "=r"(t[10]),
-                   "=r"(t[11]), "=r"(t[12]), "=r"(t[13]), "=r"(t[14]), "=r"(t[15])
-                 : "r"(address));
-}
-template<>
-__device__ __forceinline__ void load_accumulator<32>(uint32_t (&t)[32], uint32_t address)
-{
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(t[0]), "=r"(t[1]), "=r"(t[2]), "=r"(t[3]), "=r"(t[4]), "=r"(t[5]), "=r"(t[6]), "=r"(t[7]), "=r"(t[8]), "=r"(t[9]), "=r"(t[10]), "=r"(t[11]),
-          "=r"(t[12]), "=r"(t[13]), "=r"(t[14]), "=r"(t[15]), "=r"(t[16]), "=r"(t[17]), "=r"(t[18]), "=r"(t[19]), "=r"(t[20]), "=r"(t[21]), "=r"(t[22]),
-          "=r"(t[23]), "=r"(t[24]), "=r"(t[25]), "=r"(t[26]), "=r"(t[27]), "=r"(t[28]), "=r"(t[29]), "=r"(t[30]), "=r"(t[31])
-        : "r"(address));
-}
-// The registers go through the wait, so that nothing that uses them moves in front of it.
-template<int kCount>
-__device__ __forceinline__ void wait_accumulator(uint32_t (&t)[kCount]);
-template<>
-__device__ __forceinline__ void wait_accumulator<16>(uint32_t (&t)[16])
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(t[0]), "+r"(t[1]), "+r"(t[2]), "+r"(t[3]), "+r"(t[4]), "+r"(t[5]), "+r"(t[6]), "+r"(t[7]), "+r"(t[8]), "+r"(t[9]), "+r"(t[10]),
-                   "+r"(t[11]), "+r"(t[12]), "+r"(t[13]), "+r"(t[14]), "+r"(t[15])::"memory");
-}
-template<>
-__device__ __forceinline__ void wait_accumulator<32>(uint32_t (&t)[32])
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(t[0]), "+r"(t[1]), "+r"(t[2]), "+r"(t[3]), "+r"(t[4]), "+r"(t[5]), "+r"(t[6]), "+r"(t[7]), "+r"(t[8]), "+r"(t[9]), "+r"(t[10]), "+r"(t[11]),
-                   "+r"(t[12]), "+r"(t[13]), "+r"(t[14]), "+r"(t[15]), "+r"(t[16]), "+r"(t[17]), "+r"(t[18]), "+r"(t[19]), "+r"(t[20]), "+r"(t[21]), "+r"(t[22]),
-                   "+r"(t[23]), "+r"(t[24]), "+r"(t[25]), "+r"(t[26]), "+r"(t[27]), "+r"(t[28]), "+r"(t[29]), "+r"(t[30]), "+r"(t[31])::"memory");
-}
-// two sums at once: sum += part * factor
-__device__ __forceinline__ void add_scaled_pair(uint64_t& sum, uint32_t part_low, uint32_t part_high, uint64_t factors)
-{
-    asm("{\n"
-        ".reg .b64 part;\n"
-        "mov.b64 part, {%1, %2};\n"
-        "fma.rn.f32x2 %0, part, %3, %0;\n"
-        "}\n"
-        : "+l"(sum)
-        : "r"(part_low), "r"(part_high), "l"(factors));
-}
-
-// One thread of a whole warp.  Not a comparison of the lane: behind that the compiler feeds every instruction of the tensor
-// cores and the copy engine through code for several lanes (a block of 128 columns took about 1000 cycles to issue).
-__device__ __forceinline__ bool elect_one()
-{
-    uint32_t elected;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "elect.sync _|p, 0xFFFFFFFF;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(elected));
-    return elected != 0u;
-}
+constexpr uint32_t kRoleThreads = 128;  // four warps that copy and issue; those that sum come behind them
 
 // ---- tiles ------------------------------------------------------------------------------
 
@@ -195,13 +32,13 @@ struct Tile
     uint32_t expert;
     uint32_t first_row;
     uint32_t rows;
-    uint32_t output_block;
+    uint32_t output_tile;
 };
 
 // The tile-th tile of the call.  first_tile: [experts + 1] tiles before each expert's.  Within an expert, groups of row tiles
 // share a weight tile before the next weight tile is taken: a wave of CTAs then reads a few of both from L2.
-template<int kTokens>
-__device__ __forceinline__ Tile find_tile(const ProductArgs& a, const uint32_t* first_tile, uint32_t tile, uint32_t output_blocks)
+template<uint32_t kRows>
+__device__ __forceinline__ Tile find_tile(const ProductArgs& a, const uint32_t* first_tile, uint32_t tile, uint32_t output_tiles)
 {
     Tile found;
     uint32_t low = 0, high = a.expert_count;
@@ -216,25 +53,24 @@ __device__ __forceinline__ Tile find_tile(const ProductArgs& a, const uint32_t* 
     found.expert = low;
     const uint32_t begin = a.expert_offsets != nullptr ? a.expert_offsets[low] : 0u;
     const uint32_t end = a.expert_offsets != nullptr ? a.expert_offsets[low + 1u] : a.rows;
-    const uint32_t row_tiles = (end - begin + kTokens - 1u) / kTokens;
+    const uint32_t row_tiles = (end - begin + kRows - 1u) / kRows;
     const uint32_t local = tile - first_tile[low];
-    const uint32_t group = local / (kGroupTiles * output_blocks);
-    const uint32_t in_group = local - group * kGroupTiles * output_blocks;
+    const uint32_t group = local / (kGroupTiles * output_tiles);
+    const uint32_t in_group = local - group * kGroupTiles * output_tiles;
     const uint32_t width = min(kGroupTiles, row_tiles - group * kGroupTiles);
-    found.output_block = in_group / width;
-    const uint32_t row_tile = group * kGroupTiles + in_group - found.output_block * width;
-    found.first_row = begin + row_tile * kTokens;
-    found.rows = min(static_cast<uint32_t>(kTokens), end - found.first_row);
+    found.output_tile = in_group / width;
+    const uint32_t row_tile = group * kGroupTiles + in_group - found.output_tile * width;
+    found.first_row = begin + row_tile * kRows;
+    found.rows = min(kRows, end - found.first_row);
     return found;
 }
 
 // Tiles before every expert's, by all threads; returns false when the offsets descend or exceed the rows.
-template<int kTokens>
-__device__ __forceinline__ bool count_tiles(const ProductArgs& a, uint32_t* first_tile, uint32_t output_blocks)
+template<uint32_t kRows>
+__device__ __forceinline__ bool count_tiles(const ProductArgs& a, uint32_t* first_tile, uint32_t output_tiles)
 {
     __shared__ uint32_t warp_totals[32];
-    const uint32_t threads = Shape<kTokens>::kThreads;
-    const uint32_t per = (a.expert_count + threads - 1u) / threads;
+    const uint32_t per = (a.expert_count + blockDim.x - 1u) / blockDim.x;
     const uint32_t begin = min(a.expert_count, threadIdx.x * per), end = min(a.expert_count, begin + per);
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     bool good = true;
@@ -244,7 +80,7 @@ __device__ __forceinline__ bool count_tiles(const ProductArgs& a, uint32_t* firs
         const uint32_t first = a.expert_offsets != nullptr ? a.expert_offsets[e] : 0u;
         const uint32_t last = a.expert_offsets != nullptr ? a.expert_offsets[e + 1u] : a.rows;
         good = good && first <= last && last <= a.rows;
-        mine += (last - first + kTokens - 1u) / kTokens * output_blocks;
+        mine += (last - first + kRows - 1u) / kRows * output_tiles;
     }
     uint32_t before = mine;
 #pragma unroll
@@ -266,61 +102,136 @@ __device__ __forceinline__ bool count_tiles(const ProductArgs& a, uint32_t* firs
         const uint32_t first = a.expert_offsets != nullptr ? a.expert_offsets[e] : 0u;
         const uint32_t last = a.expert_offsets != nullptr ? a.expert_offsets[e + 1u] : a.rows;
         first_tile[e] = before;
-        before += (last - first + kTokens - 1u) / kTokens * output_blocks;
+        before += (last - first + kRows - 1u) / kRows * output_tiles;
     }
     if (end == a.expert_count && begin < end)
         first_tile[a.expert_count] = before;
     return true;
 }
 
-// ---- the kernel -------------------------------------------------------------------------
+// ---- roles that both kernels have ----------------------------------------------------------
 
-// A position in a ring of `size` slots: its slot and the parity of the phase that it is in.
-struct Cursor
+// No copy may land after the CTA has left: the last ones are waited for, in the order of their requests.
+__device__ __forceinline__ void wait_for_copies(uint32_t full, const Cursor& cursor, uint32_t stages, uint32_t issued)
 {
-    uint32_t slot = 0;
-    uint32_t parity = 0;
-    __device__ __forceinline__ void advance(uint32_t size)
+    for (uint32_t back = min(issued, stages); back > 0u; --back)
     {
-        if (++slot == size)
+        const uint32_t slot = (cursor.slot + stages - back) % stages;
+        const uint32_t parity = slot < cursor.slot ? cursor.parity : cursor.parity ^ 1u;
+        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(full + 8u * slot, parity); ++spin)
+            ;
+    }
+}
+
+struct ProductRings
+{
+    uint32_t stages; // operand tiles: the tall one (lanes), then the wide one (columns)
+    uint32_t full;
+    uint32_t empty;
+    uint32_t sum_full;
+    uint32_t sum_empty;
+};
+
+// Issues the products of every kThreads-th block, beginning with the thread's own.  One thread.
+template<bool kPair, uint32_t kStages, uint32_t kStageBytes, uint32_t kAccumulators, uint32_t kWide, uint32_t kThreads>
+__device__ __forceinline__ void issue_products(const ProductRings& rings, uint32_t memory_base, uint32_t tiles, uint32_t first, uint32_t stride, uint32_t columns,
+                                               uint32_t thread, volatile uint32_t* stalled)
+{
+    constexpr uint32_t kDescriptor = product_descriptor(kPair ? 2u * kLanes : kLanes, kWide);
+    const uint32_t blocks = (columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    Cursor cursor, sum;
+    uint32_t turn = 0;
+    uint32_t last_slot = 0, last_parity = 0;
+    bool running = true, any = false;
+    for (uint32_t t = first; t < tiles && running; t += stride)
+    {
+        for (uint32_t block = 0; block < blocks; ++block)
         {
-            slot = 0;
-            parity ^= 1u;
+            if (turn == thread)
+            {
+                running = barrier_wait(rings.sum_empty + 8u * sum.slot, sum.parity ^ 1u, stalled) && barrier_wait(rings.full + 8u * cursor.slot, cursor.parity, stalled);
+                if (!running)
+                    break;
+                memory_fence_after();
+                const uint32_t stage = rings.stages + cursor.slot * kStageBytes;
+                const uint64_t tall = tile_descriptor(stage), wide = tile_descriptor(stage + kTallTile);
+                // what lies behind the last column is zero: whole steps of it are left out
+                const uint32_t steps = min(4u, (columns - block * MOE_EXPERT_BLOCK + 31u) / 32u);
+#pragma unroll
+                for (uint32_t step = 0; step < 4u; ++step)
+                    if (step < steps)
+                        issue_product<kPair>(memory_base + sum.slot * kWide, tall + 2u * step, wide + 2u * step, kDescriptor, step != 0u);
+                commit_products<kPair>(rings.empty + 8u * cursor.slot);
+                commit_products<kPair>(rings.sum_full + 8u * sum.slot);
+                any = true;
+                last_slot = sum.slot;
+                last_parity = sum.parity;
+            }
+            turn = turn + 1u == kThreads ? 0u : turn + 1u;
+            cursor.advance(kStages);
+            sum.advance(kAccumulators);
         }
     }
+    // tensor memory is given back at the end: the last product must be done, also when somebody stalled
+    if (any)
+        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(rings.sum_full + 8u * last_slot, last_parity); ++spin)
+            ;
+}
+
+// ---- few rows an expert ----------------------------------------------------------------------
+
+constexpr uint32_t kScaleGroup = 4; // blocks whose scales are passed on together
+constexpr uint32_t kScaleSlots = 2; // groups of scales that wait for the sums
+
+template<int kTokens>
+struct FewShape
+{
+    static constexpr uint32_t kStageBytes = kTallTile + kTokens * kBlockBytes;
+    static constexpr uint32_t kStages = kTokens <= 16 ? 10u : kTokens <= 32 ? 9u : kTokens <= 64 ? 8u : 6u;
+    static constexpr uint32_t kAccumulators = 4;
+    static constexpr uint32_t kMemoryColumns = kTokens * kAccumulators;
+    static constexpr uint32_t kSumWarps = kTokens <= 64 ? 4u : 8u;
+    static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
+    static constexpr uint32_t kColumns = kTokens / (kSumWarps / 4u);    // columns of the tile that a warp sums
+    static constexpr uint32_t kChunk = kColumns < 32u ? kColumns : 32u; // columns read from tensor memory at once
+    static constexpr uint32_t kScaleBytes = kScaleSlots * kScaleGroup * kTokens * 4u;
+    static constexpr uint32_t kRawGroupBytes = kScaleGroup * kTokens * 4u + 128u; // scales of a group as they were copied, the weights' behind the rows'
+    static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators + 2u * kScaleSlots;
+    static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kScaleBytes + 2u * kRawGroupBytes + kBarriers * 8u + 64u;
 };
 
 template<int kTokens, typename Out>
-__global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
-    expert_product_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
+__global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
+    expert_product_few_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
 {
-    using S = Shape<kTokens>;
+    using S = FewShape<kTokens>;
     extern __shared__ unsigned char shared_raw[];
     __shared__ uint32_t memory_base_shared;
     __shared__ volatile uint32_t stalled;
     unsigned char* const shared = shared_raw + ((1024u - (shared_address(shared_raw) & 1023u)) & 1023u);
-    const uint32_t stages = shared_address(shared);
-    const uint32_t scale_slots = stages + S::kStages * S::kStageBytes;
-    const uint32_t full = scale_slots + S::kScaleBytes;
-    const uint32_t empty = full + 8u * S::kStages;
-    const uint32_t sum_full = empty + 8u * S::kStages;
-    const uint32_t sum_empty = sum_full + 8u * S::kAccumulators;
-    const uint32_t scale_full = sum_empty + 8u * S::kAccumulators;
+    ProductRings rings;
+    rings.stages = shared_address(shared);
+    const uint32_t scale_slots = rings.stages + S::kStages * S::kStageBytes;
+    rings.full = scale_slots + S::kScaleBytes + 2u * S::kRawGroupBytes;
+    rings.empty = rings.full + 8u * S::kStages;
+    rings.sum_full = rings.empty + 8u * S::kStages;
+    rings.sum_empty = rings.sum_full + 8u * S::kAccumulators;
+    const uint32_t scale_full = rings.sum_empty + 8u * S::kAccumulators;
     const uint32_t scale_empty = scale_full + 8u * kScaleSlots;
-    uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + S::kScaleBytes + 8u * S::kBarriers);
+    uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + S::kScaleBytes + 2u * S::kRawGroupBytes + 8u * S::kBarriers);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0)
     {
         for (uint32_t i = 0; i < S::kStages; ++i)
         {
-            barrier_init(full + 8u * i, 1u);
-            barrier_init(empty + 8u * i, 1u);
+            barrier_init(rings.full + 8u * i, 1u);
+            barrier_init(rings.empty + 8u * i, 1u);
         }
         for (uint32_t i = 0; i < S::kAccumulators; ++i)
         {
-            barrier_init(sum_full + 8u * i, 1u);
-            barrier_init(sum_empty + 8u * i, S::kSumWarps);
+            barrier_init(rings.sum_full + 8u * i, 1u);
+            barrier_init(rings.sum_empty + 8u * i, S::kSumWarps);
         }
         for (uint32_t i = 0; i < kScaleSlots; ++i)
         {
@@ -328,22 +239,17 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
             barrier_init(scale_empty + 8u * i, S::kSumWarps);
         }
         stalled = 0u;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        barrier_init_fence();
     }
     if (warp == 3u)
-    {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&memory_base_shared)), "r"(S::kMemoryColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        allocate_memory<false>(shared_address(&memory_base_shared), S::kMemoryColumns);
+    memory_sync<false>();
     const uint32_t memory_base = memory_base_shared;
 
     wait_for_previous_kernel();
     const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
-    const uint32_t output_blocks = (a.outputs + kOutputs - 1u) / kOutputs;
-    const bool good = count_tiles<kTokens>(a, first_tile, output_blocks);
+    const uint32_t output_tiles = (a.outputs + kLanes - 1u) / kLanes; // blocks of the weights' scales, too
+    const bool good = count_tiles<kTokens>(a, first_tile, output_tiles);
     __syncthreads();
     const uint32_t tiles = good ? first_tile[a.expert_count] : 0u;
     if (!good && threadIdx.x == 0)
@@ -357,183 +263,178 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
             uint32_t issued = 0;
             for (uint32_t t = blockIdx.x; t < tiles && stalled == 0u; t += gridDim.x)
             {
-                const Tile tile = find_tile<kTokens>(a, first_tile, t, output_blocks);
-                const uint32_t weight_row = tile.expert * a.outputs + tile.output_block * kOutputs;
+                const Tile tile = find_tile<kTokens>(a, first_tile, t, output_tiles);
+                // past an expert's last output lie the next one's weights, and zeros behind the last row: neither is stored
+                const uint32_t weight_row = tile.expert * a.outputs + tile.output_tile * kLanes;
                 for (uint32_t block = 0; block < blocks; ++block)
                 {
-                    if (!barrier_wait(empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled))
+                    if (!barrier_wait(rings.empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled))
                         break;
-                    const uint32_t stage = stages + cursor.slot * S::kStageBytes;
-                    const uint32_t barrier = full + 8u * cursor.slot;
+                    const uint32_t stage = rings.stages + cursor.slot * S::kStageBytes;
+                    const uint32_t barrier = rings.full + 8u * cursor.slot;
                     barrier_expect_bytes(barrier, S::kStageBytes);
-                    copy_tile(stage, &weight_map, block * kBlockBytes, weight_row, barrier);
-                    copy_tile(stage + kWeightTile, &row_map, block * kBlockBytes, tile.first_row, barrier);
+                    copy_tile<false>(stage, &weight_map, block * kBlockBytes, weight_row, barrier);
+                    copy_tile<false>(stage + kTallTile, &row_map, block * kBlockBytes, tile.first_row, barrier);
                     cursor.advance(S::kStages);
                     ++issued;
                 }
             }
-            // no copy may land after the CTA has left: the last ones are waited for, in the order of their requests
-            for (uint32_t back = min(issued, S::kStages); back > 0u; --back)
-            {
-                const uint32_t slot = (cursor.slot + S::kStages - back) % S::kStages;
-                const uint32_t parity = slot < cursor.slot ? cursor.parity : cursor.parity ^ 1u;
-                for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(full + 8u * slot, parity); ++spin)
-                    ;
-            }
+            wait_for_copies(rings.full, cursor, S::kStages, issued);
         }
     }
     else if (warp == 1u)
     {
         if (elect_one())
-        {
-            Cursor cursor, sum;
-            bool running = true;
-            bool any = false;
-            for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
-            {
-                for (uint32_t block = 0; block < blocks; ++block)
-                {
-                    running = barrier_wait(sum_empty + 8u * sum.slot, sum.parity ^ 1u, &stalled) && barrier_wait(full + 8u * cursor.slot, cursor.parity, &stalled);
-                    if (!running)
-                        break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t stage = stages + cursor.slot * S::kStageBytes;
-                    const uint64_t weights = tile_descriptor(stage), rows = tile_descriptor(stage + kWeightTile);
-                    // what lies behind the last column is zero: whole steps of it are left out
-                    const uint32_t steps = min(4u, (a.columns - block * MOE_EXPERT_BLOCK + 31u) / 32u);
-                    for (uint32_t step = 0; step < steps; ++step)
-                        issue_product(memory_base + sum.slot * kTokens, weights + 2u * step, rows + 2u * step, product_descriptor<kTokens>(), step != 0u);
-                    commit_products(empty + 8u * cursor.slot);
-                    commit_products(sum_full + 8u * sum.slot);
-                    any = true;
-                    cursor.advance(S::kStages);
-                    sum.advance(S::kAccumulators);
-                }
-            }
-            // tensor memory is given back below: the last product must be done, also when somebody stalled
-            if (any)
-            {
-                const uint32_t slot = sum.slot == 0u ? S::kAccumulators - 1u : sum.slot - 1u;
-                const uint32_t parity = sum.slot == 0u ? sum.parity ^ 1u : sum.parity;
-                for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(sum_full + 8u * slot, parity); ++spin)
-                    ;
-            }
-        }
+            issue_products<false, S::kStages, S::kStageBytes, S::kAccumulators, kTokens, 1u>(rings, memory_base, tiles, blockIdx.x, gridDim.x, a.columns, 0u, &stalled);
     }
     else if (warp == 2u)
     {
-        // The products of the scales, four blocks ahead of the ring in registers.
+        // The products of the scales, four blocks at a time: the scales of the group behind this one are on their way (also those
+        // of the next tile) while this group's are multiplied.
         constexpr uint32_t kPerLane = (kTokens + 31u) / 32u;
-        constexpr uint32_t kAhead = 4;
-        Cursor cursor;
-        bool running = true;
-        for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
-        {
-            const Tile tile = find_tile<kTokens>(a, first_tile, t, output_blocks);
-            const float* weight_scales = a.weight_scales + (static_cast<size_t>(tile.expert) * output_blocks + tile.output_block) * blocks;
-            const float* scales = a.scales + tile.first_row;
-            float next[kAhead][kPerLane], next_weight[kAhead];
-            const auto load = [&](uint32_t first) {
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i)
+        const uint32_t raw_slots = scale_slots + S::kScaleBytes;
+        uint32_t ahead_tile = blockIdx.x, ahead_block = 0, ahead_slot = 0;
+        const float* ahead_scales = nullptr;
+        const float* ahead_weights = nullptr;
+        uint32_t ahead_rows = 0;
+        const auto request = [&]() {
+            if (ahead_tile < tiles)
+            {
+                if (ahead_block == 0u)
                 {
-                    const uint32_t block = first + i;
-                    next_weight[i] = block < blocks ? weight_scales[block] : 0.0f;
+                    const Tile tile = find_tile<kTokens>(a, first_tile, ahead_tile, output_tiles);
+                    ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_tiles + tile.output_tile) * blocks;
+                    ahead_scales = a.scales + tile.first_row;
+                    ahead_rows = tile.rows;
+                }
+                const uint32_t raw = raw_slots + ahead_slot * S::kRawGroupBytes + 4u * lane;
+                const uint32_t count = min(kScaleGroup, blocks - ahead_block);
 #pragma unroll
-                    for (uint32_t j = 0; j < kPerLane; ++j)
+                for (uint32_t i = 0; i < kScaleGroup; ++i)
+                {
+                    if (i < count)
                     {
-                        const uint32_t row = lane + 32u * j;
-                        next[i][j] = block < blocks && row < tile.rows ? scales[static_cast<size_t>(block) * a.rows + row] : 0.0f;
+#pragma unroll
+                        for (uint32_t j = 0; j < kPerLane; ++j)
+                        {
+                            const uint32_t row = lane + 32u * j;
+                            if (kTokens >= 32 || lane < kTokens)
+                                copy_word(raw + (i * kTokens + 32u * j) * 4u, ahead_scales + (row < ahead_rows ? row : 0u), row < ahead_rows);
+                        }
+                        ahead_scales += a.rows;
                     }
                 }
-            };
-            load(0u);
-            for (uint32_t first = 0; first < blocks && running; first += kAhead)
-            {
-                float now[kAhead][kPerLane];
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i)
-#pragma unroll
-                    for (uint32_t j = 0; j < kPerLane; ++j)
-                        now[i][j] = next[i][j] * next_weight[i];
-                if (first + kAhead < blocks)
-                    load(first + kAhead);
-#pragma unroll
-                for (uint32_t i = 0; i < kAhead; ++i)
+                if (lane < count)
+                    copy_word(raw + kScaleGroup * kTokens * 4u, ahead_weights + ahead_block + lane, true);
+                ahead_block += count;
+                if (ahead_block == blocks)
                 {
-                    if (first + i >= blocks || !running)
-                        break;
-                    running = __all_sync(kFullMask, barrier_wait(scale_empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled)) != 0;
-                    if (!running)
-                        break;
-                    const uint32_t slot = scale_slots + cursor.slot * kTokens * 4u;
+                    ahead_block = 0;
+                    ahead_tile += gridDim.x;
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ahead_slot ^= 1u;
+        };
+        Cursor cursor;
+        uint32_t raw_slot = 0;
+        bool running = true;
+        request();
+        for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
+        {
+            for (uint32_t block = 0; block < blocks; block += kScaleGroup)
+            {
+                request();
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                __syncwarp(); // the weights' scales are other lanes' copies
+                running = barrier_wait_warp(scale_empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled);
+                if (!running)
+                    break;
+                const uint32_t raw = raw_slots + raw_slot * S::kRawGroupBytes;
+                const uint32_t slot = scale_slots + cursor.slot * kScaleGroup * kTokens * 4u + 4u * lane;
+                // (blocks behind the last one: what an earlier group left there, which nobody reads)
+                const uint4 weights = load_shared_16(raw + kScaleGroup * kTokens * 4u);
+                const float weight[kScaleGroup] = {__uint_as_float(weights.x), __uint_as_float(weights.y), __uint_as_float(weights.z), __uint_as_float(weights.w)};
+#pragma unroll
+                for (uint32_t i = 0; i < kScaleGroup; ++i)
+                {
 #pragma unroll
                     for (uint32_t j = 0; j < kPerLane; ++j)
                         if (kTokens >= 32 || lane < kTokens)
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + 4u * (lane + 32u * j)), "f"(now[i][j]) : "memory");
-                    __syncwarp();
-                    if (lane == 0u)
-                        barrier_arrive(scale_full + 8u * cursor.slot);
-                    cursor.advance(kScaleSlots);
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (i * kTokens + 32u * j) * 4u),
+                                         "f"(__uint_as_float(load_shared_32(raw + (i * kTokens + 32u * j + lane) * 4u)) * weight[i])
+                                         : "memory");
                 }
+                __syncwarp();
+                if (lane == 0u)
+                    barrier_arrive(scale_full + 8u * cursor.slot);
+                cursor.advance(kScaleSlots);
+                raw_slot ^= 1u;
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     }
     else if (warp >= 4u)
     {
-        const uint32_t quarter = warp & 3u;                                // lanes of tensor memory that this warp can read
-        const uint32_t first_column = (warp - 4u) / 4u * S::kColumns;      // columns of the tile that it sums
+        const uint32_t quarter = warp & 3u;                           // lanes of tensor memory that this warp can read
+        const uint32_t first_column = (warp - 4u) / 4u * S::kColumns; // columns of the tile that it sums
         const uint32_t memory = memory_base + (quarter << 21) + first_column;
         Cursor sum, scale;
         bool running = true;
         for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
         {
-            uint64_t sums[S::kColumns / 2];
+            float sums[S::kColumns];
 #pragma unroll
-            for (uint32_t i = 0; i < S::kColumns / 2; ++i)
-                sums[i] = 0ull;
+            for (uint32_t i = 0; i < S::kColumns; ++i)
+                sums[i] = 0.0f;
             for (uint32_t block = 0; block < blocks; ++block)
             {
-                running = __all_sync(kFullMask, barrier_wait(scale_full + 8u * scale.slot, scale.parity, &stalled) &&
-                                                    barrier_wait(sum_full + 8u * sum.slot, sum.parity, &stalled)) != 0;
+                const uint32_t in_group = block % kScaleGroup;
+                running = (in_group != 0u || barrier_wait_warp(scale_full + 8u * scale.slot, scale.parity, &stalled)) &&
+                          barrier_wait_warp(rings.sum_full + 8u * sum.slot, sum.parity, &stalled);
                 if (!running)
                     break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t factors = scale_slots + (scale.slot * kTokens + first_column) * 4u;
+                memory_fence_after();
+                const uint32_t factors = scale_slots + ((scale.slot * kScaleGroup + in_group) * kTokens + first_column) * 4u;
                 const uint32_t source = memory + sum.slot * kTokens;
-                // the next chunk is on its way while this one is summed
+                // at most two chunks, on their way together
                 constexpr uint32_t kChunks = S::kColumns / S::kChunk;
-                uint32_t part[2][S::kChunk];
-                load_accumulator<S::kChunk>(part[0], source);
+                static_assert(kChunks <= 2u, "an accumulator is read with two requests");
+                uint32_t part[kChunks][S::kChunk];
 #pragma unroll
                 for (uint32_t chunk = 0; chunk < kChunks; ++chunk)
-                {
-                    wait_accumulator<S::kChunk>(part[chunk & 1u]);
-                    if (chunk + 1u < kChunks)
-                        load_accumulator<S::kChunk>(part[(chunk + 1u) & 1u], source + (chunk + 1u) * S::kChunk);
+                    load_accumulator<S::kChunk>(part[chunk], source + chunk * S::kChunk);
 #pragma unroll
-                    for (uint32_t i = 0; i < S::kChunk; i += 4u)
-                    {
-                        const ulonglong2 factor = load_shared_2x64(factors + (chunk * S::kChunk + i) * 4u);
-                        const uint32_t(&p)[S::kChunk] = part[chunk & 1u];
-                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u], p[i], p[i + 1u], factor.x);
-                        add_scaled_pair(sums[(chunk * S::kChunk + i) / 2u + 1u], p[i + 2u], p[i + 3u], factor.y);
-                    }
-                }
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                for (uint32_t chunk = 0; chunk < kChunks; ++chunk)
+                    wait_accumulator<S::kChunk>(part[chunk]);
+                // all of it is in registers: the accumulator may be written again
+                memory_fence_before();
                 __syncwarp();
                 if (lane == 0u)
+                    barrier_arrive(rings.sum_empty + 8u * sum.slot);
+#pragma unroll
+                for (uint32_t i = 0; i < S::kColumns; i += 4u)
                 {
-                    barrier_arrive(sum_empty + 8u * sum.slot);
-                    barrier_arrive(scale_empty + 8u * scale.slot);
+                    const uint4 factor = load_shared_16(factors + i * 4u);
+                    const uint32_t* p = part[i / S::kChunk] + i % S::kChunk;
+                    sums[i] = fmaf(__uint_as_float(p[0]), __uint_as_float(factor.x), sums[i]);
+                    sums[i + 1u] = fmaf(__uint_as_float(p[1]), __uint_as_float(factor.y), sums[i + 1u]);
+                    sums[i + 2u] = fmaf(__uint_as_float(p[2]), __uint_as_float(factor.z), sums[i + 2u]);
+                    sums[i + 3u] = fmaf(__uint_as_float(p[3]), __uint_as_float(factor.w), sums[i + 3u]);
                 }
                 sum.advance(S::kAccumulators);
-                scale.advance(kScaleSlots);
+                if (in_group + 1u == kScaleGroup || block + 1u == blocks)
+                {
+                    __syncwarp();
+                    if (lane == 0u)
+                        barrier_arrive(scale_empty + 8u * scale.slot);
+                    scale.advance(kScaleSlots);
+                }
             }
             if (!running)
                 break;
-            const Tile tile = find_tile<kTokens>(a, first_tile, t, output_blocks);
-            const uint32_t output = tile.output_block * kOutputs + quarter * 32u + lane;
+            const Tile tile = find_tile<kTokens>(a, first_tile, t, output_tiles);
+            const uint32_t output = tile.output_tile * kLanes + quarter * 32u + lane;
             if (output < a.outputs)
             {
                 Out* target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + first_column) * a.out_stride + output;
@@ -542,7 +443,7 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
                 {
                     if (first_column + i < tile.rows)
                     {
-                        const float value = __uint_as_float(static_cast<uint32_t>(sums[i / 2u] >> (32u * (i & 1u))));
+                        const float value = sums[i];
                         if constexpr (sizeof(Out) == 4)
                             target[static_cast<size_t>(i) * a.out_stride] = value;
                         else
@@ -552,14 +453,297 @@ __global__ void __launch_bounds__(Shape<kTokens>::kThreads, 1)
             }
         }
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    memory_sync<false>();
     if (warp == 3u)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(memory_base), "r"(S::kMemoryColumns) : "memory");
+        free_memory<false>(memory_base, S::kMemoryColumns);
     if (threadIdx.x == 0 && stalled != 0u)
         atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
 }
+
+// ---- many rows an expert ---------------------------------------------------------------------
+
+constexpr uint32_t kTileOutputs = 256;
+
+// kPair: two CTAs of a cluster share a tile of 256 rows.  Each has its 128 rows and the weights of half of the outputs in its
+// shared memory; the first one issues products that read both halves and write both tensor memories.
+template<bool kPair>
+struct ManyShape
+{
+    static constexpr uint32_t kCtas = kPair ? 2u : 1u;
+    static constexpr uint32_t kTileRows = kLanes * kCtas;
+    static constexpr uint32_t kWeightBox = kTileOutputs / kCtas; // weight rows that a CTA copies
+    static constexpr uint32_t kStageBytes = kTallTile + kWeightBox * kBlockBytes;
+    static constexpr uint32_t kStages = kPair ? 6u : 4u;
+    static constexpr uint32_t kAccumulators = 2;
+    static constexpr uint32_t kMemoryColumns = kTileOutputs * kAccumulators;
+    static constexpr uint32_t kIssuers = 1;
+    static constexpr uint32_t kSumWarps = 8;
+    static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
+    static constexpr uint32_t kColumns = kTileOutputs / 2u; // outputs that a warp sums: one block of the weights' scales
+    static constexpr uint32_t kChunk = 32;
+    static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators;
+    static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kBarriers * 8u + 64u;
+    // 128 sums in a thread: the warps that sum take registers over from the other roles.  Launched with 168 a thread:
+    // 128 * 56 + 256 * 224 = 384 * 168.
+    static constexpr uint32_t kRoleRegisters = 56;
+    static constexpr uint32_t kSumRegisters = 224;
+};
+
+// Sixteen bytes of outputs of one row.
+__device__ __forceinline__ void store_outputs(float* target, const float* values)
+{
+    *reinterpret_cast<float4*>(target) = make_float4(values[0], values[1], values[2], values[3]);
+}
+__device__ __forceinline__ void store_outputs(__nv_bfloat16* target, const float* values)
+{
+    uint32_t words[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(values[2 * i], values[2 * i + 1]);
+        words[i] = *reinterpret_cast<const uint32_t*>(&pair);
+    }
+    *reinterpret_cast<uint4*>(target) = make_uint4(words[0], words[1], words[2], words[3]);
+}
+__device__ __forceinline__ void store_output(float* target, float value)
+{
+    *target = value;
+}
+__device__ __forceinline__ void store_output(__nv_bfloat16* target, float value)
+{
+    *target = __float2bfloat16_rn(value);
+}
+
+template<bool kPair, typename Out>
+__global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
+    expert_product_many_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
+{
+    using S = ManyShape<kPair>;
+    extern __shared__ unsigned char shared_raw[];
+    __shared__ uint32_t memory_base_shared;
+    __shared__ volatile uint32_t stalled;
+    unsigned char* const shared = shared_raw + ((1024u - (shared_address(shared_raw) & 1023u)) & 1023u);
+    ProductRings rings;
+    rings.stages = shared_address(shared);
+    rings.full = rings.stages + S::kStages * S::kStageBytes;
+    rings.empty = rings.full + 8u * S::kStages;
+    rings.sum_full = rings.empty + 8u * S::kStages;
+    rings.sum_empty = rings.sum_full + 8u * S::kAccumulators;
+    uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + 8u * S::kBarriers);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t cta = kPair ? cta_in_cluster() : 0u; // of the pair
+
+    if (threadIdx.x == 0)
+    {
+        for (uint32_t i = 0; i < S::kStages; ++i)
+        {
+            barrier_init(rings.full + 8u * i, 1u);
+            barrier_init(rings.empty + 8u * i, 1u);
+        }
+        for (uint32_t i = 0; i < S::kAccumulators; ++i)
+        {
+            barrier_init(rings.sum_full + 8u * i, 1u);
+            barrier_init(rings.sum_empty + 8u * i, S::kSumWarps * S::kCtas);
+        }
+        stalled = 0u;
+        barrier_init_fence();
+    }
+    __syncwarp();
+    if (warp == 3u)
+        allocate_memory<kPair>(shared_address(&memory_base_shared), S::kMemoryColumns);
+    memory_sync<kPair>();
+    const uint32_t memory_base = memory_base_shared;
+
+    wait_for_previous_kernel();
+    const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    const uint32_t output_blocks = (a.outputs + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    const uint32_t output_tiles = (a.outputs + kTileOutputs - 1u) / kTileOutputs;
+    const bool good = count_tiles<S::kTileRows>(a, first_tile, output_tiles);
+    __syncthreads();
+    const uint32_t tiles = good ? first_tile[a.expert_count] : 0u;
+    if (!good && threadIdx.x == 0)
+        atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
+    const uint32_t first = blockIdx.x / S::kCtas, stride = gridDim.x / S::kCtas;
+
+    if (warp < 4u)
+    {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRoleRegisters));
+        if (warp == 0u)
+        {
+            if (elect_one())
+            {
+                Cursor cursor;
+                uint32_t issued = 0;
+                for (uint32_t t = first; t < tiles && stalled == 0u; t += stride)
+                {
+                    const Tile tile = find_tile<S::kTileRows>(a, first_tile, t, output_tiles);
+                    // what lies past an expert's rows or outputs belongs to the next one, or is zero: it is not stored
+                    const uint32_t weight_row = tile.expert * a.outputs + tile.output_tile * kTileOutputs + cta * S::kWeightBox;
+                    const uint32_t row = tile.first_row + cta * kLanes;
+                    for (uint32_t block = 0; block < blocks; ++block)
+                    {
+                        if (!barrier_wait(rings.empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled))
+                            break;
+                        const uint32_t stage = rings.stages + cursor.slot * S::kStageBytes;
+                        uint32_t barrier = rings.full + 8u * cursor.slot;
+                        if (cta == 0u)
+                            barrier_expect_bytes(barrier, S::kStageBytes * S::kCtas);
+                        else
+                            barrier = barrier_of_cta(barrier, 0u);
+                        copy_tile<kPair>(stage, &row_map, block * kBlockBytes, row, barrier);
+                        copy_tile<kPair>(stage + kTallTile, &weight_map, block * kBlockBytes, weight_row, barrier);
+                        cursor.advance(S::kStages);
+                        ++issued;
+                    }
+                }
+                // (The second CTA of a pair has seen its copies used, or a wait run out that is far longer than a copy takes.)
+                if (cta == 0u)
+                    wait_for_copies(rings.full, cursor, S::kStages, issued);
+            }
+        }
+        else if (warp <= S::kIssuers)
+        {
+            // Two threads take turns: between two blocks a thread spends longer on its barriers than the tensor cores have
+            // products left in their queue.
+            if (cta == 0u)
+                if (elect_one())
+                    issue_products<kPair, S::kStages, S::kStageBytes, S::kAccumulators, kTileOutputs, S::kIssuers>(rings, memory_base, tiles, first, stride, a.columns, warp - 1u, &stalled);
+        }
+    }
+    else
+    {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSumRegisters));
+        const uint32_t quarter = warp & 3u;      // lanes of tensor memory that this warp can read
+        const uint32_t half = (warp - 4u) / 4u;  // of the tile's outputs
+        const uint32_t memory = memory_base + (quarter << 21) + half * S::kColumns;
+        const uint32_t row = cta * kLanes + quarter * 32u + lane; // of a tile
+        // The scales are read two blocks ahead, across tiles.
+        uint32_t ahead_tile = first, ahead_block = 0;
+        const float* ahead_scales = nullptr;
+        const float* ahead_weights = nullptr;
+        float next_scale[2], next_weight[2];
+        const auto request = [&]() {
+            if (ahead_tile < tiles)
+            {
+                if (ahead_block == 0u)
+                {
+                    const Tile tile = find_tile<S::kTileRows>(a, first_tile, ahead_tile, output_tiles);
+                    // (an odd number of blocks: the second half of the last tile has no scales, and is not stored)
+                    const uint32_t output_block = min(tile.output_tile * 2u + half, output_blocks - 1u);
+                    ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_blocks + output_block) * blocks;
+                    ahead_scales = a.scales + tile.first_row + (row < tile.rows ? row : 0u);
+                }
+                const uint32_t second = ahead_block + 1u < blocks ? 1u : 0u;
+                next_scale[0] = ahead_scales[0];
+                next_weight[0] = ahead_weights[ahead_block];
+                next_scale[1] = ahead_scales[second != 0u ? a.rows : 0u];
+                next_weight[1] = ahead_weights[ahead_block + second];
+                ahead_scales += 2u * static_cast<size_t>(a.rows);
+                ahead_block += 2u;
+                if (ahead_block >= blocks)
+                {
+                    ahead_block = 0;
+                    ahead_tile += stride;
+                }
+            }
+        };
+        request();
+        Cursor sum;
+        bool running = true;
+        for (uint32_t t = first; t < tiles && running; t += stride)
+        {
+            float sums[S::kColumns];
+#pragma unroll
+            for (uint32_t i = 0; i < S::kColumns; ++i)
+                sums[i] = 0.0f;
+            for (uint32_t block = 0; block < blocks && running; block += 2u)
+            {
+                const float factors[2] = {next_scale[0] * next_weight[0], next_scale[1] * next_weight[1]};
+                request();
+#pragma unroll
+                for (uint32_t of_two = 0; of_two < 2u; ++of_two)
+                {
+                    if (block + of_two >= blocks)
+                        break;
+                    running = barrier_wait_warp(rings.sum_full + 8u * sum.slot, sum.parity, &stalled);
+                    if (!running)
+                        break;
+                    memory_fence_after();
+                    const uint32_t source = memory + sum.slot * kTileOutputs;
+                    const float factor = factors[of_two];
+                    // Two chunks are on their way at a time, and the next two are requested as these are summed: while products
+                    // run, tensor memory serves half as much to warps with one request outstanding.  (Single adds: the pairs of
+                    // fma.f32x2 would have to be moved together first.)
+                    constexpr uint32_t kChunks = S::kColumns / S::kChunk;
+                    uint32_t part[2][S::kChunk];
+                    load_accumulator<S::kChunk>(part[0], source);
+                    load_accumulator<S::kChunk>(part[1], source + S::kChunk);
+#pragma unroll
+                    for (uint32_t chunk = 0; chunk < kChunks; ++chunk)
+                    {
+                        if (chunk % 2u == 0u)
+                        {
+                            wait_accumulator<S::kChunk>(part[0]);
+                            wait_accumulator<S::kChunk>(part[1]);
+                            if (chunk + 2u >= kChunks)
+                            {
+                                // all of it is in registers: the accumulator may be written again
+                                memory_fence_before();
+                                __syncwarp();
+                                if (lane == 0u)
+                                {
+                                    if (cta == 0u)
+                                        barrier_arrive(rings.sum_empty + 8u * sum.slot);
+                                    else
+                                        barrier_arrive_cluster(barrier_of_cta(rings.sum_empty + 8u * sum.slot, 0u));
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t i = 0; i < S::kChunk; ++i)
+                            sums[chunk * S::kChunk + i] = fmaf(__uint_as_float(part[chunk & 1u][i]), factor, sums[chunk * S::kChunk + i]);
+                        if (chunk + 2u < kChunks)
+                            load_accumulator<S::kChunk>(part[chunk & 1u], source + (chunk + 2u) * S::kChunk);
+                    }
+                    sum.advance(S::kAccumulators);
+                }
+            }
+            if (!running)
+                break;
+            const Tile tile = find_tile<S::kTileRows>(a, first_tile, t, output_tiles);
+            const uint32_t output = tile.output_tile * kTileOutputs + half * S::kColumns;
+            if (row < tile.rows && output < a.outputs)
+            {
+                constexpr uint32_t kVector = 16u / sizeof(Out);
+                Out* target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + row) * a.out_stride + output;
+                const uint32_t count = min(S::kColumns, a.outputs - output);
+                const bool vector = (reinterpret_cast<uintptr_t>(a.out) | (a.out_stride * sizeof(Out))) % 16u == 0u;
+#pragma unroll
+                for (uint32_t i = 0; i < S::kColumns; i += kVector)
+                {
+                    float values[kVector];
+#pragma unroll
+                    for (uint32_t j = 0; j < kVector; ++j)
+                        values[j] = sums[i + j];
+                    if (vector && i + kVector <= count)
+                        store_outputs(target + i, values);
+                    else
+#pragma unroll
+                        for (uint32_t j = 0; j < kVector; ++j)
+                            if (i + j < count)
+                                store_output(target + i + j, values[j]);
+                }
+            }
+        }
+    }
+    memory_sync<kPair>(); // neither side's shared or tensor memory is used any more
+    if (warp == 3u)
+        free_memory<kPair>(memory_base, S::kMemoryColumns);
+    if (threadIdx.x == 0 && stalled != 0u)
+        atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
+}
+
+// ---- launches -------------------------------------------------------------------------------
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -588,35 +772,69 @@ bool encode_rows(CUtensorMap* map, const uint8_t* base, uint32_t columns, uint64
                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template<int kTokens, typename Out>
-cudaError_t launch_tiles(const ProductArgs& a, int sm_count, cudaStream_t stream)
+template<typename Kernel>
+cudaError_t launch_tiles(Kernel kernel, SharedOptIn& opt_in, const ProductArgs& a, uint32_t tile_rows, uint32_t tile_outputs, uint32_t row_box, uint32_t weight_box,
+                         uint32_t ctas, uint32_t threads, size_t fixed_bytes, int sm_count, cudaStream_t stream)
 {
-    using S = Shape<kTokens>;
     CUtensorMap weight_map, row_map;
-    if (!encode_rows(&weight_map, a.weights, a.columns, static_cast<uint64_t>(a.expert_count) * a.outputs, kOutputs) ||
-        !encode_rows(&row_map, a.values, a.columns, a.rows, kTokens))
+    if (!encode_rows(&weight_map, a.weights, a.columns, static_cast<uint64_t>(a.expert_count) * a.outputs, weight_box) ||
+        !encode_rows(&row_map, a.values, a.columns, a.rows, row_box))
         return cudaErrorInvalidValue;
-    const uint64_t row_tiles = (static_cast<uint64_t>(a.rows) + kTokens - 1u) / kTokens + (a.expert_count < a.rows ? a.expert_count : a.rows) - 1u;
-    const uint64_t tiles = row_tiles * ((a.outputs + kOutputs - 1u) / kOutputs);
-    const size_t shared_bytes = 1024u + S::kFixedBytes + sizeof(uint32_t) * (static_cast<size_t>(a.expert_count) + 1u);
-    static SharedOptIn opt_in;
-    if (cudaError_t status = opt_in_shared(opt_in, expert_product_kernel<kTokens, Out>, shared_bytes))
+    // the most row tiles that any offsets give
+    const uint64_t row_tiles = (static_cast<uint64_t>(a.rows) + tile_rows - 1u) / tile_rows + (a.expert_count < a.rows ? a.expert_count : a.rows) - 1u;
+    const uint64_t tiles = row_tiles * ((a.outputs + tile_outputs - 1u) / tile_outputs);
+    const size_t shared_bytes = 1024u + fixed_bytes + sizeof(uint32_t) * (static_cast<size_t>(a.expert_count) + 1u);
+    if (cudaError_t status = opt_in_shared(opt_in, kernel, shared_bytes))
         return status;
-    const uint32_t grid = static_cast<uint32_t>(tiles < static_cast<uint64_t>(sm_count) ? tiles : static_cast<uint64_t>(sm_count));
-    return launch_following(expert_product_kernel<kTokens, Out>, grid, S::kThreads, shared_bytes, stream, a, weight_map, row_map);
+    const uint64_t most = static_cast<uint64_t>(sm_count) / ctas;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<uint32_t>((tiles < most ? tiles : most) * ctas), 1, 1);
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = shared_bytes;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2] = {follow_closely(), {}};
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = ctas;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = ctas > 1u ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, a, weight_map, row_map);
+}
+
+template<int kTokens, typename Out>
+cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
+{
+    using S = FewShape<kTokens>;
+    static SharedOptIn opt_in;
+    return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, kTokens, kLanes, 1u, S::kThreads, S::kFixedBytes, sm_count, stream);
+}
+template<bool kPair, typename Out>
+cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
+{
+    using S = ManyShape<kPair>;
+    static SharedOptIn opt_in;
+    return launch_tiles(expert_product_many_kernel<kPair, Out>, opt_in, a, S::kTileRows, kTileOutputs, kLanes, S::kWeightBox, S::kCtas, S::kThreads, S::kFixedBytes, sm_count,
+                        stream);
 }
 
 template<typename Out>
 cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
     const uint32_t per_expert = (a.rows + a.expert_count - 1u) / a.expert_count;
+#ifdef FORCE
+    if (per_expert > 16u)
+        return FORCE;
+#endif
     if (per_expert <= 16u)
-        return launch_tiles<16, Out>(a, sm_count, stream);
+        return launch_few<16, Out>(a, sm_count, stream);
     if (per_expert <= 32u)
-        return launch_tiles<32, Out>(a, sm_count, stream);
+        return launch_few<32, Out>(a, sm_count, stream);
     if (per_expert <= 64u)
-        return launch_tiles<64, Out>(a, sm_count, stream);
-    return launch_tiles<128, Out>(a, sm_count, stream);
+        return launch_few<64, Out>(a, sm_count, stream);
+    if (per_expert <= 192u)
+        return launch_many<false, Out>(a, sm_count, stream);
+    return launch_many<true, Out>(a, sm_count, stream);
 }
 
 } // namespace
