@@ -132,50 +132,42 @@ struct ProductRings
     uint32_t sum_empty;
 };
 
-// Issues the products of every kThreads-th block, beginning with the thread's own.  One thread.
-template<bool kPair, uint32_t kStages, uint32_t kStageBytes, uint32_t kAccumulators, uint32_t kWide, uint32_t kThreads>
-__device__ __forceinline__ void issue_products(const ProductRings& rings, uint32_t memory_base, uint32_t tiles, uint32_t first, uint32_t stride, uint32_t columns,
-                                               uint32_t thread, volatile uint32_t* stalled)
+// Issues the products of `count` blocks in a row, the first of them block `block` of its tile.  One thread.
+template<bool kPair, uint32_t kStages, uint32_t kStageBytes, uint32_t kAccumulators, uint32_t kWide>
+__device__ __forceinline__ void issue_products(const ProductRings& rings, uint32_t memory_base, uint32_t count, uint32_t block, uint32_t columns, volatile uint32_t* stalled)
 {
     constexpr uint32_t kDescriptor = product_descriptor(kPair ? 2u * kLanes : kLanes, kWide);
     const uint32_t blocks = (columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    const uint32_t last_steps = (columns - (blocks - 1u) * MOE_EXPERT_BLOCK + 31u) / 32u;
     Cursor cursor, sum;
-    uint32_t turn = 0;
-    uint32_t last_slot = 0, last_parity = 0;
-    bool running = true, any = false;
-    for (uint32_t t = first; t < tiles && running; t += stride)
+    uint32_t done = 0;
+    for (; done < count; ++done)
     {
-        for (uint32_t block = 0; block < blocks; ++block)
-        {
-            if (turn == thread)
-            {
-                running = barrier_wait(rings.sum_empty + 8u * sum.slot, sum.parity ^ 1u, stalled) && barrier_wait(rings.full + 8u * cursor.slot, cursor.parity, stalled);
-                if (!running)
-                    break;
-                memory_fence_after();
-                const uint32_t stage = rings.stages + cursor.slot * kStageBytes;
-                const uint64_t tall = tile_descriptor(stage), wide = tile_descriptor(stage + kTallTile);
-                // what lies behind the last column is zero: whole steps of it are left out
-                const uint32_t steps = min(4u, (columns - block * MOE_EXPERT_BLOCK + 31u) / 32u);
+        if (!barrier_wait(rings.sum_empty + 8u * sum.slot, sum.parity ^ 1u, stalled) || !barrier_wait(rings.full + 8u * cursor.slot, cursor.parity, stalled))
+            break;
+        memory_fence_after();
+        const uint32_t stage = rings.stages + cursor.slot * kStageBytes;
+        const uint64_t tall = tile_descriptor(stage), wide = tile_descriptor(stage + kTallTile);
+        // what lies behind the last column is zero: whole steps of it are left out
+        const uint32_t steps = ++block == blocks ? last_steps : 4u;
+        block = block == blocks ? 0u : block;
 #pragma unroll
-                for (uint32_t step = 0; step < 4u; ++step)
-                    if (step < steps)
-                        issue_product<kPair>(memory_base + sum.slot * kWide, tall + 2u * step, wide + 2u * step, kDescriptor, step != 0u);
-                commit_products<kPair>(rings.empty + 8u * cursor.slot);
-                commit_products<kPair>(rings.sum_full + 8u * sum.slot);
-                any = true;
-                last_slot = sum.slot;
-                last_parity = sum.parity;
-            }
-            turn = turn + 1u == kThreads ? 0u : turn + 1u;
-            cursor.advance(kStages);
-            sum.advance(kAccumulators);
-        }
+        for (uint32_t step = 0; step < 4u; ++step)
+            if (step < steps)
+                issue_product<kPair>(memory_base + sum.slot * kWide, tall + 2u * step, wide + 2u * step, kDescriptor, step != 0u);
+        commit_products<kPair>(rings.empty + 8u * cursor.slot);
+        commit_products<kPair>(rings.sum_full + 8u * sum.slot);
+        cursor.advance(kStages);
+        sum.advance(kAccumulators);
     }
     // tensor memory is given back at the end: the last product must be done, also when somebody stalled
-    if (any)
-        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(rings.sum_full + 8u * last_slot, last_parity); ++spin)
+    if (done > 0u)
+    {
+        const uint32_t slot = sum.slot == 0u ? kAccumulators - 1u : sum.slot - 1u;
+        const uint32_t parity = sum.slot == 0u ? sum.parity ^ 1u : sum.parity;
+        for (uint32_t spin = 0; spin < kSpinLimit && !barrier_test(rings.sum_full + 8u * slot, parity); ++spin)
             ;
+    }
 }
 
 // ---- few rows an expert ----------------------------------------------------------------------
@@ -187,22 +179,45 @@ template<int kTokens>
 struct FewShape
 {
     static constexpr uint32_t kStageBytes = kTallTile + kTokens * kBlockBytes;
-    static constexpr uint32_t kStages = kTokens <= 16 ? 10u : kTokens <= 32 ? 9u : kTokens <= 64 ? 8u : 6u;
+    static constexpr uint32_t kStages = kTokens <= 16 ? 10u : kTokens <= 32 ? 9u : 8u;
     static constexpr uint32_t kAccumulators = 4;
     static constexpr uint32_t kMemoryColumns = kTokens * kAccumulators;
-    static constexpr uint32_t kSumWarps = kTokens <= 64 ? 4u : 8u;
+    static constexpr uint32_t kSumWarps = 4;
     static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
-    static constexpr uint32_t kColumns = kTokens / (kSumWarps / 4u);    // columns of the tile that a warp sums
-    static constexpr uint32_t kChunk = kColumns < 32u ? kColumns : 32u; // columns read from tensor memory at once
+    static constexpr uint32_t kChunk = kTokens < 32 ? kTokens : 32; // columns read from tensor memory at once
     static constexpr uint32_t kScaleBytes = kScaleSlots * kScaleGroup * kTokens * 4u;
     static constexpr uint32_t kRawGroupBytes = kScaleGroup * kTokens * 4u + 128u; // scales of a group as they were copied, the weights' behind the rows'
     static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators + 2u * kScaleSlots;
     static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kScaleBytes + 2u * kRawGroupBytes + kBarriers * 8u + 64u;
 };
 
+// a float in another CTA's shared memory
+__device__ __forceinline__ float load_shared_of_cta(uint32_t address, uint32_t cta)
+{
+    float value;
+    asm volatile(
+        "{\n"
+        ".reg .u32 remote;\n"
+        "mapa.shared::cluster.u32 remote, %1, %2;\n"
+        "ld.shared::cluster.f32 %0, [remote];\n"
+        "}\n"
+        : "=f"(value)
+        : "r"(address), "r"(cta)
+        : "memory");
+    return value;
+}
+__device__ __forceinline__ void store_output(float* target, float value)
+{
+    *target = value;
+}
+__device__ __forceinline__ void store_output(__nv_bfloat16* target, float value)
+{
+    *target = __float2bfloat16_rn(value);
+}
+
 template<int kTokens, typename Out>
 __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
-    expert_product_few_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
+    expert_product_few_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map, const uint32_t split)
 {
     using S = FewShape<kTokens>;
     extern __shared__ unsigned char shared_raw[];
@@ -254,6 +269,10 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
     const uint32_t tiles = good ? first_tile[a.expert_count] : 0u;
     if (!good && threadIdx.x == 0)
         atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
+    // With a split, a cluster has one tile and each of its CTAs a part of the columns.
+    const uint32_t cta = split > 1u ? cta_in_cluster() : 0u;
+    const uint32_t first = blockIdx.x / split, stride = gridDim.x / split;
+    const uint32_t begin = blocks * cta / split, end = blocks * (cta + 1u) / split;
 
     if (warp == 0u)
     {
@@ -261,12 +280,12 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
         {
             Cursor cursor;
             uint32_t issued = 0;
-            for (uint32_t t = blockIdx.x; t < tiles && stalled == 0u; t += gridDim.x)
+            for (uint32_t t = first; t < tiles && stalled == 0u; t += stride)
             {
                 const Tile tile = find_tile<kTokens>(a, first_tile, t, output_tiles);
                 // past an expert's last output lie the next one's weights, and zeros behind the last row: neither is stored
                 const uint32_t weight_row = tile.expert * a.outputs + tile.output_tile * kLanes;
-                for (uint32_t block = 0; block < blocks; ++block)
+                for (uint32_t block = begin; block < end; ++block)
                 {
                     if (!barrier_wait(rings.empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled))
                         break;
@@ -285,30 +304,32 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
     else if (warp == 1u)
     {
         if (elect_one())
-            issue_products<false, S::kStages, S::kStageBytes, S::kAccumulators, kTokens, 1u>(rings, memory_base, tiles, blockIdx.x, gridDim.x, a.columns, 0u, &stalled);
+            issue_products<false, S::kStages, S::kStageBytes, S::kAccumulators, kTokens>(
+                rings, memory_base, first < tiles ? ((tiles - first - 1u) / stride + 1u) * (end - begin) : 0u, begin, a.columns, &stalled);
     }
     else if (warp == 2u)
     {
-        // The products of the scales, four blocks at a time: the scales of the group behind this one are on their way (also those
-        // of the next tile) while this group's are multiplied.
+        // The products of the scales, up to four blocks of a tile at a time: the scales of the group behind this one are on their
+        // way (also those of the next tile) while this group's are multiplied.
         constexpr uint32_t kPerLane = (kTokens + 31u) / 32u;
         const uint32_t raw_slots = scale_slots + S::kScaleBytes;
-        uint32_t ahead_tile = blockIdx.x, ahead_block = 0, ahead_slot = 0;
+        uint32_t ahead_tile = begin < end ? first : tiles, ahead_slot = 0, ahead_left = 0; // its blocks that are left
         const float* ahead_scales = nullptr;
         const float* ahead_weights = nullptr;
         uint32_t ahead_rows = 0;
         const auto request = [&]() {
             if (ahead_tile < tiles)
             {
-                if (ahead_block == 0u)
+                if (ahead_left == 0u)
                 {
                     const Tile tile = find_tile<kTokens>(a, first_tile, ahead_tile, output_tiles);
-                    ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_tiles + tile.output_tile) * blocks;
-                    ahead_scales = a.scales + tile.first_row;
+                    ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_tiles + tile.output_tile) * blocks + begin;
+                    ahead_scales = a.scales + static_cast<size_t>(begin) * a.rows + tile.first_row;
                     ahead_rows = tile.rows;
+                    ahead_left = end - begin;
                 }
                 const uint32_t raw = raw_slots + ahead_slot * S::kRawGroupBytes + 4u * lane;
-                const uint32_t count = min(kScaleGroup, blocks - ahead_block);
+                const uint32_t count = min(kScaleGroup, ahead_left);
 #pragma unroll
                 for (uint32_t i = 0; i < kScaleGroup; ++i)
                 {
@@ -325,24 +346,22 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
                     }
                 }
                 if (lane < count)
-                    copy_word(raw + kScaleGroup * kTokens * 4u, ahead_weights + ahead_block + lane, true);
-                ahead_block += count;
-                if (ahead_block == blocks)
-                {
-                    ahead_block = 0;
-                    ahead_tile += gridDim.x;
-                }
+                    copy_word(raw + kScaleGroup * kTokens * 4u, ahead_weights + lane, true);
+                ahead_weights += count;
+                ahead_left -= count;
+                if (ahead_left == 0u)
+                    ahead_tile += stride;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             ahead_slot ^= 1u;
         };
         Cursor cursor;
         uint32_t raw_slot = 0;
-        bool running = true;
         request();
-        for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
+        bool running = true;
+        for (uint32_t t = first; t < tiles && running; t += stride)
         {
-            for (uint32_t block = 0; block < blocks; block += kScaleGroup)
+            for (uint32_t block = begin; block < end; block += kScaleGroup)
             {
                 request();
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -355,10 +374,10 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
                 // (blocks behind the last one: what an earlier group left there, which nobody reads)
                 const uint4 weights = load_shared_16(raw + kScaleGroup * kTokens * 4u);
                 const float weight[kScaleGroup] = {__uint_as_float(weights.x), __uint_as_float(weights.y), __uint_as_float(weights.z), __uint_as_float(weights.w)};
-#pragma unroll
+    #pragma unroll
                 for (uint32_t i = 0; i < kScaleGroup; ++i)
                 {
-#pragma unroll
+    #pragma unroll
                     for (uint32_t j = 0; j < kPerLane; ++j)
                         if (kTokens >= 32 || lane < kTokens)
                             asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot + (i * kTokens + 32u * j) * 4u),
@@ -376,29 +395,29 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
     }
     else if (warp >= 4u)
     {
-        const uint32_t quarter = warp & 3u;                           // lanes of tensor memory that this warp can read
-        const uint32_t first_column = (warp - 4u) / 4u * S::kColumns; // columns of the tile that it sums
-        const uint32_t memory = memory_base + (quarter << 21) + first_column;
+        const uint32_t quarter = warp & 3u; // lanes of tensor memory that this warp can read
+        const uint32_t memory = memory_base + (quarter << 21);
+        const uint32_t tile_lane = quarter * 32u + lane;
         Cursor sum, scale;
         bool running = true;
-        for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
+        for (uint32_t t = first; t < tiles && running; t += stride)
         {
-            float sums[S::kColumns];
+            float sums[kTokens];
 #pragma unroll
-            for (uint32_t i = 0; i < S::kColumns; ++i)
+            for (uint32_t i = 0; i < kTokens; ++i)
                 sums[i] = 0.0f;
-            for (uint32_t block = 0; block < blocks; ++block)
+            for (uint32_t block = begin; block < end; ++block)
             {
-                const uint32_t in_group = block % kScaleGroup;
+                const uint32_t in_group = (block - begin) % kScaleGroup;
                 running = (in_group != 0u || barrier_wait_warp(scale_full + 8u * scale.slot, scale.parity, &stalled)) &&
                           barrier_wait_warp(rings.sum_full + 8u * sum.slot, sum.parity, &stalled);
                 if (!running)
                     break;
                 memory_fence_after();
-                const uint32_t factors = scale_slots + ((scale.slot * kScaleGroup + in_group) * kTokens + first_column) * 4u;
+                const uint32_t factors = scale_slots + (scale.slot * kScaleGroup + in_group) * kTokens * 4u;
                 const uint32_t source = memory + sum.slot * kTokens;
                 // at most two chunks, on their way together
-                constexpr uint32_t kChunks = S::kColumns / S::kChunk;
+                constexpr uint32_t kChunks = kTokens / S::kChunk;
                 static_assert(kChunks <= 2u, "an accumulator is read with two requests");
                 uint32_t part[kChunks][S::kChunk];
 #pragma unroll
@@ -413,7 +432,7 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
                 if (lane == 0u)
                     barrier_arrive(rings.sum_empty + 8u * sum.slot);
 #pragma unroll
-                for (uint32_t i = 0; i < S::kColumns; i += 4u)
+                for (uint32_t i = 0; i < kTokens; i += 4u)
                 {
                     const uint4 factor = load_shared_16(factors + i * 4u);
                     const uint32_t* p = part[i / S::kChunk] + i % S::kChunk;
@@ -423,7 +442,7 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
                     sums[i + 3u] = fmaf(__uint_as_float(p[3]), __uint_as_float(factor.w), sums[i + 3u]);
                 }
                 sum.advance(S::kAccumulators);
-                if (in_group + 1u == kScaleGroup || block + 1u == blocks)
+                if (in_group + 1u == kScaleGroup || block + 1u == end)
                 {
                     __syncwarp();
                     if (lane == 0u)
@@ -433,23 +452,23 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
             }
             if (!running)
                 break;
+            if (split > 1u)
+            {
+                // the cluster's parts are added below; the stages are free: the last product that read them is done
+#pragma unroll
+                for (uint32_t i = 0; i < kTokens; ++i)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(rings.stages + (i * kLanes + tile_lane) * 4u), "f"(sums[i]) : "memory");
+                break;
+            }
             const Tile tile = find_tile<kTokens>(a, first_tile, t, output_tiles);
-            const uint32_t output = tile.output_tile * kLanes + quarter * 32u + lane;
+            const uint32_t output = tile.output_tile * kLanes + tile_lane;
             if (output < a.outputs)
             {
-                Out* target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + first_column) * a.out_stride + output;
+                Out* target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row) * a.out_stride + output;
 #pragma unroll
-                for (uint32_t i = 0; i < S::kColumns; ++i)
-                {
-                    if (first_column + i < tile.rows)
-                    {
-                        const float value = sums[i];
-                        if constexpr (sizeof(Out) == 4)
-                            target[static_cast<size_t>(i) * a.out_stride] = value;
-                        else
-                            target[static_cast<size_t>(i) * a.out_stride] = __float2bfloat16_rn(value);
-                    }
-                }
+                for (uint32_t i = 0; i < kTokens; ++i)
+                    if (i < tile.rows)
+                        store_output(target + static_cast<size_t>(i) * a.out_stride, sums[i]);
             }
         }
     }
@@ -458,6 +477,27 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
         free_memory<false>(memory_base, S::kMemoryColumns);
     if (threadIdx.x == 0 && stalled != 0u)
         atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
+    if (split > 1u)
+    {
+        // Each CTA adds the parts of some of the rows, in the order of the columns.
+        cluster_sync();
+        if (warp >= 4u && first < tiles)
+        {
+            const Tile tile = find_tile<kTokens>(a, first_tile, first, output_tiles);
+            const uint32_t tile_lane = (warp & 3u) * 32u + lane;
+            const uint32_t output = tile.output_tile * kLanes + tile_lane;
+            for (uint32_t i = cta; i < tile.rows; i += split)
+            {
+                float total = 0.0f;
+                for (uint32_t part = 0; part < split; ++part)
+                    total += load_shared_of_cta(rings.stages + (i * kLanes + tile_lane) * 4u, part);
+                if (output < a.outputs)
+                    store_output(static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + i) * a.out_stride + output, total);
+            }
+        }
+        __syncwarp();
+        cluster_sync(); // nobody leaves while its part is read
+    }
 }
 
 // ---- many rows an expert ---------------------------------------------------------------------
@@ -476,7 +516,6 @@ struct ManyShape
     static constexpr uint32_t kStages = kPair ? 6u : 4u;
     static constexpr uint32_t kAccumulators = 2;
     static constexpr uint32_t kMemoryColumns = kTileOutputs * kAccumulators;
-    static constexpr uint32_t kIssuers = 1;
     static constexpr uint32_t kSumWarps = 8;
     static constexpr uint32_t kThreads = kRoleThreads + 32u * kSumWarps;
     static constexpr uint32_t kColumns = kTileOutputs / 2u; // outputs that a warp sums: one block of the weights' scales
@@ -484,9 +523,9 @@ struct ManyShape
     static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators;
     static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kBarriers * 8u + 64u;
     // 128 sums in a thread: the warps that sum take registers over from the other roles.  Launched with 168 a thread:
-    // 128 * 56 + 256 * 224 = 384 * 168.
-    static constexpr uint32_t kRoleRegisters = 56;
-    static constexpr uint32_t kSumRegisters = 224;
+    // 128 * 40 + 256 * 232 = 384 * 168.
+    static constexpr uint32_t kRoleRegisters = 40;
+    static constexpr uint32_t kSumRegisters = 232;
 };
 
 // Sixteen bytes of outputs of one row.
@@ -505,15 +544,6 @@ __device__ __forceinline__ void store_outputs(__nv_bfloat16* target, const float
     }
     *reinterpret_cast<uint4*>(target) = make_uint4(words[0], words[1], words[2], words[3]);
 }
-__device__ __forceinline__ void store_output(float* target, float value)
-{
-    *target = value;
-}
-__device__ __forceinline__ void store_output(__nv_bfloat16* target, float value)
-{
-    *target = __float2bfloat16_rn(value);
-}
-
 template<bool kPair, typename Out>
 __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
     expert_product_many_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
@@ -601,13 +631,12 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
                     wait_for_copies(rings.full, cursor, S::kStages, issued);
             }
         }
-        else if (warp <= S::kIssuers)
+        else if (warp == 1u)
         {
-            // Two threads take turns: between two blocks a thread spends longer on its barriers than the tensor cores have
-            // products left in their queue.
             if (cta == 0u)
                 if (elect_one())
-                    issue_products<kPair, S::kStages, S::kStageBytes, S::kAccumulators, kTileOutputs, S::kIssuers>(rings, memory_base, tiles, first, stride, a.columns, warp - 1u, &stalled);
+                    issue_products<kPair, S::kStages, S::kStageBytes, S::kAccumulators, kTileOutputs>(
+                        rings, memory_base, first < tiles ? ((tiles - first - 1u) / stride + 1u) * blocks : 0u, 0u, a.columns, &stalled);
         }
     }
     else
@@ -617,37 +646,44 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
         const uint32_t half = (warp - 4u) / 4u;  // of the tile's outputs
         const uint32_t memory = memory_base + (quarter << 21) + half * S::kColumns;
         const uint32_t row = cta * kLanes + quarter * 32u + lane; // of a tile
-        // The scales are read two blocks ahead, across tiles.
+        // The scales are read two blocks ahead, across tiles.  The loads stand outside of any condition (behind the last tile they
+        // repeat the last ones): a value that is merged with another one behind a branch is waited for there.
         uint32_t ahead_tile = first, ahead_block = 0;
-        const float* ahead_scales = nullptr;
-        const float* ahead_weights = nullptr;
+        const float* ahead_scales = a.scales;
+        const float* ahead_weights = a.weight_scales;
         float next_scale[2], next_weight[2];
-        const auto request = [&]() {
+        const auto find_scales = [&]() {
             if (ahead_tile < tiles)
             {
-                if (ahead_block == 0u)
-                {
-                    const Tile tile = find_tile<S::kTileRows>(a, first_tile, ahead_tile, output_tiles);
-                    // (an odd number of blocks: the second half of the last tile has no scales, and is not stored)
-                    const uint32_t output_block = min(tile.output_tile * 2u + half, output_blocks - 1u);
-                    ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_blocks + output_block) * blocks;
-                    ahead_scales = a.scales + tile.first_row + (row < tile.rows ? row : 0u);
-                }
-                const uint32_t second = ahead_block + 1u < blocks ? 1u : 0u;
-                next_scale[0] = ahead_scales[0];
-                next_weight[0] = ahead_weights[ahead_block];
-                next_scale[1] = ahead_scales[second != 0u ? a.rows : 0u];
-                next_weight[1] = ahead_weights[ahead_block + second];
-                ahead_scales += 2u * static_cast<size_t>(a.rows);
-                ahead_block += 2u;
-                if (ahead_block >= blocks)
-                {
-                    ahead_block = 0;
-                    ahead_tile += stride;
-                }
+                const Tile tile = find_tile<S::kTileRows>(a, first_tile, ahead_tile, output_tiles);
+                // (an odd number of blocks: the second half of the last tile has no scales, and is not stored)
+                const uint32_t output_block = min(tile.output_tile * 2u + half, output_blocks - 1u);
+                ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_blocks + output_block) * blocks;
+                ahead_scales = a.scales + tile.first_row + (row < tile.rows ? row : 0u);
             }
         };
-        request();
+        const auto request = [&]() {
+            const bool second = ahead_block + 1u < blocks;
+            next_scale[0] = ahead_scales[0];
+            next_weight[0] = ahead_weights[0];
+            next_scale[1] = ahead_scales[second ? a.rows : 0u];
+            next_weight[1] = ahead_weights[second ? 1u : 0u];
+            ahead_block += 2u;
+            if (ahead_block < blocks)
+            {
+                ahead_scales += 2u * static_cast<size_t>(a.rows);
+                ahead_weights += 2u;
+            }
+            else
+            {
+                ahead_block = 0;
+                ahead_tile += stride;
+                find_scales();
+            }
+        };
+        find_scales();
+        if (first < tiles)
+            request();
         Cursor sum;
         bool running = true;
         for (uint32_t t = first; t < tiles && running; t += stride)
@@ -772,60 +808,66 @@ bool encode_rows(CUtensorMap* map, const uint8_t* base, uint32_t columns, uint64
                                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template<typename Kernel>
-cudaError_t launch_tiles(Kernel kernel, SharedOptIn& opt_in, const ProductArgs& a, uint32_t tile_rows, uint32_t tile_outputs, uint32_t row_box, uint32_t weight_box,
-                         uint32_t ctas, uint32_t threads, size_t fixed_bytes, int sm_count, cudaStream_t stream)
+template<typename... Parameters>
+cudaError_t launch_tiles(void (*kernel)(ProductArgs, CUtensorMap, CUtensorMap, Parameters...), SharedOptIn& opt_in, const ProductArgs& a, uint32_t row_box, uint32_t weight_box,
+                         uint64_t ctas, uint32_t cluster, uint32_t threads, size_t fixed_bytes, cudaStream_t stream, Parameters... more)
 {
     CUtensorMap weight_map, row_map;
     if (!encode_rows(&weight_map, a.weights, a.columns, static_cast<uint64_t>(a.expert_count) * a.outputs, weight_box) ||
         !encode_rows(&row_map, a.values, a.columns, a.rows, row_box))
         return cudaErrorInvalidValue;
-    // the most row tiles that any offsets give
-    const uint64_t row_tiles = (static_cast<uint64_t>(a.rows) + tile_rows - 1u) / tile_rows + (a.expert_count < a.rows ? a.expert_count : a.rows) - 1u;
-    const uint64_t tiles = row_tiles * ((a.outputs + tile_outputs - 1u) / tile_outputs);
     const size_t shared_bytes = 1024u + fixed_bytes + sizeof(uint32_t) * (static_cast<size_t>(a.expert_count) + 1u);
     if (cudaError_t status = opt_in_shared(opt_in, kernel, shared_bytes))
         return status;
-    const uint64_t most = static_cast<uint64_t>(sm_count) / ctas;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<uint32_t>((tiles < most ? tiles : most) * ctas), 1, 1);
+    config.gridDim = dim3(static_cast<uint32_t>(ctas), 1, 1);
     config.blockDim = dim3(threads, 1, 1);
     config.dynamicSmemBytes = shared_bytes;
     config.stream = stream;
     cudaLaunchAttribute attributes[2] = {follow_closely(), {}};
     attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = ctas;
+    attributes[1].val.clusterDim.x = cluster;
     attributes[1].val.clusterDim.y = 1;
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = ctas > 1u ? 2 : 1;
-    return cudaLaunchKernelEx(&config, kernel, a, weight_map, row_map);
+    config.numAttrs = cluster > 1u ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, a, weight_map, row_map, more...);
 }
+
+// The most tiles that any offsets give.
+uint64_t most_tiles(const ProductArgs& a, uint32_t tile_rows, uint32_t tile_outputs)
+{
+    const uint64_t row_tiles = (static_cast<uint64_t>(a.rows) + tile_rows - 1u) / tile_rows + (a.expert_count < a.rows ? a.expert_count : a.rows) - 1u;
+    return row_tiles * ((a.outputs + tile_outputs - 1u) / tile_outputs);
+}
+
+constexpr uint32_t kLeastPart = 4; // blocks of a CTA of a split tile
 
 template<int kTokens, typename Out>
 cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
     using S = FewShape<kTokens>;
     static SharedOptIn opt_in;
-    return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, kTokens, kLanes, 1u, S::kThreads, S::kFixedBytes, sm_count, stream);
+    const uint64_t tiles = most_tiles(a, kTokens, kLanes), most = static_cast<uint64_t>(sm_count);
+    const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    uint32_t split = 1;
+    while (split < 8u && tiles * split * 2u <= most && blocks >= split * 2u * kLeastPart)
+        split *= 2u;
+    return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, (tiles < most ? tiles * split : most), split, S::kThreads, S::kFixedBytes, stream, split);
 }
 template<bool kPair, typename Out>
 cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
     using S = ManyShape<kPair>;
     static SharedOptIn opt_in;
-    return launch_tiles(expert_product_many_kernel<kPair, Out>, opt_in, a, S::kTileRows, kTileOutputs, kLanes, S::kWeightBox, S::kCtas, S::kThreads, S::kFixedBytes, sm_count,
-                        stream);
+    const uint64_t tiles = most_tiles(a, S::kTileRows, kTileOutputs), most = static_cast<uint64_t>(sm_count) / S::kCtas;
+    return launch_tiles(expert_product_many_kernel<kPair, Out>, opt_in, a, kLanes, S::kWeightBox, (tiles < most ? tiles : most) * S::kCtas, S::kCtas, S::kThreads, S::kFixedBytes, stream);
 }
 
 template<typename Out>
 cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
     const uint32_t per_expert = (a.rows + a.expert_count - 1u) / a.expert_count;
-#ifdef FORCE
-    if (per_expert > 16u)
-        return FORCE;
-#endif
     if (per_expert <= 16u)
         return launch_few<16, Out>(a, sm_count, stream);
     if (per_expert <= 32u)
