@@ -174,6 +174,8 @@ __device__ __forceinline__ void issue_products(const ProductRings& rings, uint32
 
 constexpr uint32_t kScaleGroup = 4; // blocks whose scales are passed on together
 constexpr uint32_t kScaleSlots = 2; // groups of scales that wait for the sums
+constexpr uint32_t kMostParts = 8;  // CTAs that share a tile
+constexpr uint32_t kLeastPart = 4;  // blocks of each of them
 
 template<int kTokens>
 struct FewShape
@@ -191,17 +193,17 @@ struct FewShape
     static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kScaleBytes + 2u * kRawGroupBytes + kBarriers * 8u + 64u;
 };
 
-// a float in another CTA's shared memory
-__device__ __forceinline__ float load_shared_of_cta(uint32_t address, uint32_t cta)
+// four floats in another CTA's shared memory
+__device__ __forceinline__ float4 load_shared_of_cta(uint32_t address, uint32_t cta)
 {
-    float value;
+    float4 value;
     asm volatile(
         "{\n"
         ".reg .u32 remote;\n"
-        "mapa.shared::cluster.u32 remote, %1, %2;\n"
-        "ld.shared::cluster.f32 %0, [remote];\n"
+        "mapa.shared::cluster.u32 remote, %4, %5;\n"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [remote];\n"
         "}\n"
-        : "=f"(value)
+        : "=f"(value.x), "=f"(value.y), "=f"(value.z), "=f"(value.w)
         : "r"(address), "r"(cta)
         : "memory");
     return value;
@@ -479,20 +481,37 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
         atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
     if (split > 1u)
     {
-        // Each CTA adds the parts of some of the rows, in the order of the columns.
+        // Each CTA adds the parts of some of the rows, in the order of the columns: a warp a row, four outputs a lane, all parts
+        // requested before the first is added.
         cluster_sync();
-        if (warp >= 4u && first < tiles)
+        if (first < tiles)
         {
             const Tile tile = find_tile<kTokens>(a, first_tile, first, output_tiles);
-            const uint32_t tile_lane = (warp & 3u) * 32u + lane;
-            const uint32_t output = tile.output_tile * kLanes + tile_lane;
-            for (uint32_t i = cta; i < tile.rows; i += split)
+            const uint32_t output = tile.output_tile * kLanes + 4u * lane;
+            for (uint32_t i = cta + split * warp; i < tile.rows; i += split * (S::kThreads / 32u))
             {
-                float total = 0.0f;
-                for (uint32_t part = 0; part < split; ++part)
-                    total += load_shared_of_cta(rings.stages + (i * kLanes + tile_lane) * 4u, part);
-                if (output < a.outputs)
-                    store_output(static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + i) * a.out_stride + output, total);
+                float4 parts[kMostParts];
+#pragma unroll
+                for (uint32_t part = 0; part < kMostParts; ++part)
+                    if (part < split)
+                        parts[part] = load_shared_of_cta(rings.stages + (i * kLanes + 4u * lane) * 4u, part);
+                float total[4] = {parts[0].x, parts[0].y, parts[0].z, parts[0].w};
+#pragma unroll
+                for (uint32_t part = 1; part < kMostParts; ++part)
+                {
+                    if (part < split)
+                    {
+                        total[0] += parts[part].x;
+                        total[1] += parts[part].y;
+                        total[2] += parts[part].z;
+                        total[3] += parts[part].w;
+                    }
+                }
+                Out* target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + i) * a.out_stride + output;
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; ++j)
+                    if (output + j < a.outputs)
+                        store_output(target + j, total[j]);
             }
         }
         __syncwarp();
@@ -841,8 +860,6 @@ uint64_t most_tiles(const ProductArgs& a, uint32_t tile_rows, uint32_t tile_outp
     return row_tiles * ((a.outputs + tile_outputs - 1u) / tile_outputs);
 }
 
-constexpr uint32_t kLeastPart = 4; // blocks of a CTA of a split tile
-
 template<int kTokens, typename Out>
 cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
@@ -850,8 +867,10 @@ cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
     static SharedOptIn opt_in;
     const uint64_t tiles = most_tiles(a, kTokens, kLanes), most = static_cast<uint64_t>(sm_count);
     const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    // Parts of one row x 4096 x 4096 (32 tiles): 1 10.2 us, 2 8.2, 4 6.9; 64 rows x 1024 x 4096 (8 tiles) 14.7, 10.6, 8.3, 8 parts
+    // 7.7.  More than eight clusters of eight CTAs are not resident together (16 of them 14.3 us, as 32 of four 8.4).
     uint32_t split = 1;
-    while (split < 8u && tiles * split * 2u <= most && blocks >= split * 2u * kLeastPart)
+    while (split < kMostParts && tiles * split * 2u <= (split * 2u == 8u ? 64u : most) && blocks >= split * 2u * kLeastPart)
         split *= 2u;
     return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, (tiles < most ? tiles * split : most), split, S::kThreads, S::kFixedBytes, stream, split);
 }
@@ -864,19 +883,31 @@ cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
     return launch_tiles(expert_product_many_kernel<kPair, Out>, opt_in, a, kLanes, S::kWeightBox, (tiles < most ? tiles : most) * S::kCtas, S::kCtas, S::kThreads, S::kFixedBytes, stream);
 }
 
+// Experts are taken to have equal numbers of rows.  Up to 32 a tile of as many rows wastes least (64 experts of 32 rows x
+// 4096 x 4096: 32-row tiles 172 us, 64-row tiles 204, 128 x 256 tiles 187).  Above that the tiles' rates decide: a block of 64
+// rows by 128 outputs takes three fifths of the time of one of 128 by 256, so the smaller ones win while they are one wave (one
+// expert of 256 rows: 15.5 against 21.8 us) and lose from two on (512 rows: 27.0 against 22.2).  Pairs of SMs read half of
+// the weights each: that pays where many full tiles are bound by L2 (64 experts of 256 rows 367 against 420 us) and costs where
+// tiles of 256 rows are partly empty (128 rows each 351 against 211) or few (one expert of 1024 rows 24.2 against 23.0).
 template<typename Out>
 cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
-    const uint32_t per_expert = (a.rows + a.expert_count - 1u) / a.expert_count;
-    if (per_expert <= 16u)
+    const uint64_t active = a.expert_count < a.rows ? a.expert_count : a.rows;
+    const uint64_t rows = (a.rows + active - 1u) / active; // of an expert
+    if (rows <= 16u)
         return launch_few<16, Out>(a, sm_count, stream);
-    if (per_expert <= 32u)
+    if (rows <= 32u)
         return launch_few<32, Out>(a, sm_count, stream);
-    if (per_expert <= 64u)
+    const auto waves = [&](uint64_t tile_rows, uint64_t tile_outputs) {
+        const uint64_t tiles = active * ((rows + tile_rows - 1u) / tile_rows) * ((a.outputs + tile_outputs - 1u) / tile_outputs);
+        return (tiles + sm_count - 1u) / sm_count;
+    };
+    const uint64_t many = waves(kLanes, kTileOutputs);
+    if (waves(64u, kLanes) * 3u <= many * 5u)
         return launch_few<64, Out>(a, sm_count, stream);
-    if (per_expert <= 192u)
-        return launch_many<false, Out>(a, sm_count, stream);
-    return launch_many<true, Out>(a, sm_count, stream);
+    if (rows >= 224u && many >= 8u)
+        return launch_many<true, Out>(a, sm_count, stream);
+    return launch_many<false, Out>(a, sm_count, stream);
 }
 
 } // namespace
