@@ -414,7 +414,8 @@ enum moe_activation
  *              MOE_EXPERT_FLAG_TOKEN_RANGE.
  * values       device, [rows x columns] e4m3, dense
  * scales       device, [ceil(columns / 128) x rows]: block-major
- * Asynchronous on `stream`; allocates nothing. */
+ * Asynchronous on `stream`.  Calls that route their source rows twice or more on average may quantise each row once
+ * and grow the handle's scratch for that (at most 48 MiB); make the largest one before a stream capture. */
 int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,
                       int activation, const uint32_t* route_token, uint32_t route_count, uint8_t* values, float* scales);
 
@@ -447,8 +448,8 @@ int moe_expert_product(moe_sampler* sampler, void* stream, const uint8_t* values
  *              >= token_count or whose rank is >= top_k is left out and the handle remembers
  *              MOE_EXPERT_FLAG_TOKEN_RANGE; of several routes with the same token and rank the last counts.
  * base         device, [token_count x columns] of dtype, or NULL; may be `out`
- * out          device, [token_count x columns] of dtype; a token without routes gets its base, or zeros
- * Asynchronous on `stream`.  Calls with more routes than any before on this handle grow its scratch
+ * out          device, [token_count x columns] of dtype, not overlapping route_rows; a token without routes gets its base, or zeros
+ * top_k <= MOE_EXPERT_MAX_EXPERTS.  Asynchronous on `stream`.  Calls with more routes than any before on this handle grow its scratch
  * (token_count * top_k words); make the largest one before a stream capture. */
 int moe_combine_routes(moe_sampler* sampler, void* stream, const void* route_rows, int dtype, size_t row_stride, uint32_t columns,
                        const uint32_t* route_token, const uint32_t* route_rank, const float* route_weight, uint32_t route_count, uint32_t token_count,

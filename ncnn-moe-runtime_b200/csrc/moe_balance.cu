@@ -16,8 +16,10 @@ namespace moe {
 
 namespace {
 
-constexpr int kBalanceThreads = 256;
+constexpr int kBalanceThreads = 512;
 constexpr int kBalanceWarps = kBalanceThreads / 32;
+constexpr uint32_t kRegisterExperts = 1024; // up to here a lane holds a row's scores in registers
+constexpr int kWideWarps = 4;               // warps of a block for wider rows, which lie in shared memory
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -38,7 +40,7 @@ __device__ __forceinline__ float warp_max(float v)
 __device__ __forceinline__ void sigmoid_both(float x, float& value, float& rest)
 {
     const float t = expf(-fabsf(x));
-    const float large = __fdiv_rn(1.0f, 1.0f + t);
+    const float large = __fdividef(1.0f, 1.0f + t); // 1 + t is in [1, 2]: within 2 ulp
     const float small = t * large;
     value = x >= 0.0f ? large : small;
     rest = x >= 0.0f ? small : large;
@@ -53,61 +55,50 @@ __device__ __forceinline__ float sqrt_softplus(float x)
     return __fsqrt_rn(fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
 }
 
-__device__ __forceinline__ float score_of(float x, int function)
+// A score, and (kSlope) its derivative.  Softmax: exp(x - peak), which is its own derivative.
+template<int kFunction, bool kSlope>
+__device__ __forceinline__ void score_of(float x, float peak, float& score, float& slope)
 {
-    if (function == MOE_ROUTER_SQRT_SOFTPLUS)
-        return sqrt_softplus(x);
-    float value, rest;
-    sigmoid_both(x, value, rest);
-    return value;
-}
-__device__ __forceinline__ float score_slope(float x, float score, int function)
-{
-    if (function == MOE_ROUTER_SQRT_SOFTPLUS && x < -20.0f)
-        return 0.5f * score;
-    float value, rest;
-    sigmoid_both(x, value, rest);
-    return function == MOE_ROUTER_SQRT_SOFTPLUS ? __fdiv_rn(value, 2.0f * score) : value * rest;
+    if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
+    {
+        score = expf(x - peak);
+        slope = score;
+    }
+    else if constexpr (kFunction == MOE_ROUTER_SIGMOID)
+    {
+        float rest;
+        sigmoid_both(x, score, rest);
+        slope = score * rest;
+    }
+    else
+    {
+        score = sqrt_softplus(x);
+        if constexpr (kSlope)
+        {
+            float value, rest;
+            sigmoid_both(x, value, rest);
+            slope = x < -20.0f ? 0.5f * score : __fdiv_rn(value, 2.0f * score);
+        }
+    }
 }
 
-// Writes a token's scores to `row` and returns the factor that makes them sum to one (0 when they are all zero).  One warp.
-__device__ __forceinline__ float score_row(const float* logits, uint32_t experts, int function, float* row)
+__device__ __forceinline__ bool counts(const BalanceArgs& a, uint64_t token)
 {
-    const uint32_t lane = threadIdx.x & 31u;
-    float peak = 0.0f;
-    if (function == MOE_ROUTER_SOFTMAX)
-    {
-        peak = -INFINITY;
-        for (uint32_t e = lane; e < experts; e += 32u)
-            peak = fmaxf(peak, logits[e]);
-        peak = warp_max(peak);
-    }
-    float total = 0.0f;
-    for (uint32_t e = lane; e < experts; e += 32u)
-    {
-        const float score = function == MOE_ROUTER_SOFTMAX ? expf(logits[e] - peak) : score_of(logits[e], function);
-        row[e] = score;
-        total += score;
-    }
-    total = warp_sum(total);
+    return a.token_mask == nullptr || a.token_mask[token] != 0;
+}
+// what scores that sum to `total` are multiplied with; scores that are all zero stay zero
+__device__ __forceinline__ float factor_of(float total)
+{
     return total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
 }
 
-// Sums over a block's tokens: [block][expert] probabilities and counted routes, [block] counted tokens.
-__global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const BalanceArgs a)
+// ---- forward ------------------------------------------------------------------------------
+
+// Routes of counted tokens by expert, this block's share of them: whole numbers, so the order of the atomics does not matter.
+// offsets, routed: shared.  All threads; ends with a barrier before the offsets are read, not behind the counts.
+__device__ __forceinline__ void count_routes(const BalanceArgs& a, uint32_t* offsets, uint32_t* routed)
 {
-    wait_for_previous_kernel();
-    extern __shared__ __align__(16) unsigned char shared_raw[];
     const uint32_t experts = a.expert_count;
-    const uint32_t warps = blockDim.x / 32u;
-    float* rows = reinterpret_cast<float*>(shared_raw);        // [warps][experts]
-    float* sums = rows + static_cast<size_t>(warps) * experts; // [warps][experts]
-    uint32_t* routed = reinterpret_cast<uint32_t*>(sums + static_cast<size_t>(warps) * experts); // [experts]
-    uint32_t* offsets = routed + experts;                                                        // [experts + 1]
-    __shared__ uint32_t counted;
-    if (threadIdx.x == 0)
-        counted = 0u;
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint64_t most_routes = static_cast<uint64_t>(a.token_count) * a.top_k;
     bool good = true;
     for (uint32_t e = threadIdx.x; e <= experts; e += blockDim.x)
@@ -119,192 +110,454 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const 
     for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
         routed[e] = 0u;
     good = __syncthreads_and(good) != 0;
-    if (!good && threadIdx.x == 0)
-        atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
-
-    // routes of counted tokens by expert: whole numbers, so the order of the atomics does not matter
-    if (good)
+    if (!good)
     {
-        for (uint64_t route = offsets[0] + static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; route < offsets[experts];
-             route += static_cast<uint64_t>(gridDim.x) * blockDim.x)
+        if (threadIdx.x == 0)
+            atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
+        return;
+    }
+    const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
+    for (uint64_t route = offsets[0] + static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; route < offsets[experts]; route += stride)
+    {
+        const uint32_t token = a.route_token[route];
+        if (token >= a.token_count)
         {
-            const uint32_t token = a.route_token[route];
-            if (token >= a.token_count)
-            {
-                atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
-                continue;
-            }
-            if (a.token_mask != nullptr && a.token_mask[token] == 0)
-                continue;
-            uint32_t low = 0, high = experts; // the last expert whose range begins at or before the route
-            while (high - low > 1u)
-            {
-                const uint32_t middle = (low + high) / 2u;
-                if (offsets[middle] <= route)
-                    low = middle;
-                else
-                    high = middle;
-            }
-            atomicAdd(&routed[low], 1u);
-        }
-    }
-
-    float* row = rows + static_cast<size_t>(warp) * experts;
-    float* sum = sums + static_cast<size_t>(warp) * experts;
-    for (uint32_t e = lane; e < experts; e += 32u)
-        sum[e] = 0.0f;
-    uint32_t mine = 0;
-    for (uint64_t token = static_cast<uint64_t>(blockIdx.x) * warps + warp; token < a.token_count; token += static_cast<uint64_t>(gridDim.x) * warps)
-    {
-        if (a.token_mask != nullptr && a.token_mask[token] == 0)
+            atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
             continue;
-        ++mine;
-        const float factor = score_row(a.logits + token * experts, experts, a.score_function, row);
-        for (uint32_t e = lane; e < experts; e += 32u)
-            sum[e] += row[e] * factor;
+        }
+        if (!counts(a, token))
+            continue;
+        uint32_t low = 0, high = experts; // the last expert whose range begins at or before the route
+        while (high - low > 1u)
+        {
+            const uint32_t middle = (low + high) / 2u;
+            if (offsets[middle] <= route)
+                low = middle;
+            else
+                high = middle;
+        }
+        atomicAdd(&routed[low], 1u);
     }
-    if (lane == 0)
-        atomicAdd(&counted, mine);
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
-    {
-        float total = 0.0f;
-        for (uint32_t w = 0; w < warps; ++w)
-            total += sums[static_cast<size_t>(w) * experts + e];
-        a.partial_sums[static_cast<size_t>(blockIdx.x) * experts + e] = total;
-        a.partial_counts[static_cast<size_t>(blockIdx.x) * (experts + 1u) + e] = routed[e];
-    }
-    if (threadIdx.x == 0)
-        a.partial_counts[static_cast<size_t>(blockIdx.x) * (experts + 1u) + experts] = counted;
 }
 
-// The blocks' sums in block order, then the loss.
-__global__ void __launch_bounds__(1024) balance_reduce_kernel(const BalanceArgs a, uint32_t blocks)
+// The loss from every expert's sum and count; all threads of a block, expert e by the threads that hold it.
+struct LossParts
 {
-    wait_for_previous_kernel();
-    const uint32_t experts = a.expert_count;
-    __shared__ uint32_t counted_shared;
+    uint32_t counted;
+    float weighted; // this thread's share of sum c_e P_e
+};
+__device__ __forceinline__ void store_expert(const BalanceArgs& a, LossParts& parts, uint32_t expert, float sum, uint32_t count)
+{
+    const float probability = __fdiv_rn(sum, static_cast<float>(max(parts.counted, 1u)));
+    a.expert_tokens[expert] = count;
+    a.expert_probability[expert] = probability;
+    parts.weighted += static_cast<float>(count) * probability;
+}
+__device__ __forceinline__ void store_loss(const BalanceArgs& a, const LossParts& parts)
+{
     __shared__ float warp_totals[32];
-    if (threadIdx.x == 0)
-    {
-        uint32_t counted = 0;
-        for (uint32_t b = 0; b < blocks; ++b)
-            counted += a.partial_counts[static_cast<size_t>(b) * (experts + 1u) + experts];
-        counted_shared = counted;
-        a.expert_tokens[experts] = counted;
-    }
-    __syncthreads();
-    const float tokens = static_cast<float>(max(counted_shared, 1u));
-    float weighted = 0.0f;
-    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
-    {
-        float sum = 0.0f;
-        uint32_t count = 0;
-        for (uint32_t b = 0; b < blocks; ++b)
-        {
-            sum += a.partial_sums[static_cast<size_t>(b) * experts + e];
-            count += a.partial_counts[static_cast<size_t>(b) * (experts + 1u) + e];
-        }
-        const float probability = __fdiv_rn(sum, tokens);
-        a.expert_tokens[e] = count;
-        a.expert_probability[e] = probability;
-        weighted += static_cast<float>(count) * probability;
-    }
-    weighted = warp_sum(weighted);
+    const float weighted = warp_sum(parts.weighted);
     if ((threadIdx.x & 31u) == 0u)
         warp_totals[threadIdx.x >> 5] = weighted;
     __syncthreads();
     if (threadIdx.x < 32u)
     {
-        const float total = warp_sum(warp_totals[threadIdx.x]);
+        const float total = warp_sum(threadIdx.x < blockDim.x / 32u ? warp_totals[threadIdx.x] : 0.0f);
         if (threadIdx.x == 0)
-            *a.loss = a.coefficient * (total * __fdiv_rn(static_cast<float>(experts), static_cast<float>(a.top_k) * tokens));
+        {
+            const float tokens = static_cast<float>(max(parts.counted, 1u));
+            *a.loss = a.coefficient * (total * __fdiv_rn(static_cast<float>(a.expert_count), static_cast<float>(a.top_k) * tokens));
+            a.expert_tokens[a.expert_count] = parts.counted;
+        }
     }
 }
 
-__global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const BalanceArgs a, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient)
+// Sums over a block's tokens.  A warp per token: a lane has every 32nd expert, the scores and their sums over the tokens in
+// registers (kPer of each; kPer 0: in shared memory).  The blocks' sums go to scratch, or, where one block has all tokens,
+// straight into the results.
+template<int kFunction, int kPer>
+__global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const BalanceArgs a)
 {
-    wait_for_previous_kernel();
     extern __shared__ __align__(16) unsigned char shared_raw[];
     const uint32_t experts = a.expert_count;
     const uint32_t warps = blockDim.x / 32u;
-    float* shares = reinterpret_cast<float*>(shared_raw); // [experts]: g
+    uint32_t* offsets = reinterpret_cast<uint32_t*>(shared_raw); // [experts + 1]
+    uint32_t* routed = offsets + experts + 1u;                   // [experts]
+    float* sums = reinterpret_cast<float*>(routed + experts);    // [warps][experts]
+    __shared__ uint32_t counted_shared;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    float* row = shares + static_cast<size_t>(warp + 1u) * experts;
+    if (threadIdx.x == 0)
+        counted_shared = 0u;
+    wait_for_previous_kernel();
+    count_routes(a, offsets, routed);
+
+    uint32_t counted = 0;
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * warps + warp, stride = static_cast<uint64_t>(gridDim.x) * warps;
+    float* const sum_row = sums + static_cast<size_t>(warp) * experts;
+    if constexpr (kPer > 0)
+    {
+        float sum[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            sum[i] = 0.0f;
+        for (uint64_t token = first; token < a.token_count; token += stride)
+        {
+            if (!counts(a, token))
+                continue;
+            ++counted;
+            const float* logits = a.logits + token * experts;
+            float x[kPer];
+            float peak = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+            {
+                const uint32_t e = lane + 32u * i;
+                x[i] = e < experts ? logits[e] : 0.0f;
+                if (e < experts)
+                    peak = fmaxf(peak, x[i]);
+            }
+            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
+                peak = warp_max(peak);
+            float total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+            {
+                float slope;
+                score_of<kFunction, false>(x[i], peak, x[i], slope);
+                if (lane + 32u * i >= experts)
+                    x[i] = 0.0f;
+                total += x[i];
+            }
+            const float factor = factor_of(warp_sum(total));
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                sum[i] = fmaf(x[i], factor, sum[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (lane + 32u * i < experts)
+                sum_row[lane + 32u * i] = sum[i];
+    }
+    else
+    {
+        float* const row = sums + static_cast<size_t>(warps + warp) * experts; // [warps][experts] behind the sums
+        for (uint32_t e = lane; e < experts; e += 32u)
+            sum_row[e] = 0.0f;
+        for (uint64_t token = first; token < a.token_count; token += stride)
+        {
+            if (!counts(a, token))
+                continue;
+            ++counted;
+            const float* logits = a.logits + token * experts;
+            float peak = -INFINITY;
+            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
+            {
+                for (uint32_t e = lane; e < experts; e += 32u)
+                    peak = fmaxf(peak, logits[e]);
+                peak = warp_max(peak);
+            }
+            float total = 0.0f;
+            for (uint32_t e = lane; e < experts; e += 32u)
+            {
+                float score, slope;
+                score_of<kFunction, false>(logits[e], peak, score, slope);
+                row[e] = score;
+                total += score;
+            }
+            const float factor = factor_of(warp_sum(total));
+            for (uint32_t e = lane; e < experts; e += 32u)
+                sum_row[e] = fmaf(row[e], factor, sum_row[e]);
+        }
+    }
+    if (lane == 0 && counted > 0u)
+        atomicAdd(&counted_shared, counted);
+    __syncthreads();
+    LossParts parts = {counted_shared, 0.0f};
+    const bool alone = gridDim.x == 1u;
+    for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
+    {
+        float total = 0.0f;
+        for (uint32_t w = 0; w < warps; ++w)
+            total += sums[static_cast<size_t>(w) * experts + e];
+        if (alone)
+        {
+            store_expert(a, parts, e, total, routed[e]);
+        }
+        else
+        {
+            a.partial_sums[static_cast<size_t>(blockIdx.x) * experts + e] = total;
+            a.partial_counts[static_cast<size_t>(blockIdx.x) * (experts + 1u) + e] = routed[e];
+        }
+    }
+    if (alone)
+        store_loss(a, parts);
+    else if (threadIdx.x == 0)
+        a.partial_counts[static_cast<size_t>(blockIdx.x) * (experts + 1u) + experts] = parts.counted;
+}
+
+// The blocks' sums, 32 experts a CTA: a warp adds every 32nd block, then the warps' sums are added in their order.  The CTA that
+// finishes last adds the loss from all experts, in their order.
+__global__ void __launch_bounds__(1024) balance_reduce_kernel(const BalanceArgs a, uint32_t blocks)
+{
+    __shared__ float sums[32][33];
+    __shared__ uint32_t routes[32][33];
+    __shared__ uint32_t counted_shared, last_shared;
+    const uint32_t experts = a.expert_count;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t e = blockIdx.x * 32u + lane;
+    if (threadIdx.x == 0)
+        counted_shared = 0u;
+    wait_for_previous_kernel();
+    __syncthreads();
+    if (threadIdx.x < blocks)
+        atomicAdd(&counted_shared, a.partial_counts[static_cast<size_t>(threadIdx.x) * (experts + 1u) + experts]);
+    float sum = 0.0f;
+    uint32_t count = 0;
+#pragma unroll 10
+    for (uint32_t b = warp; b < blocks; b += 32u)
+    {
+        sum += e < experts ? a.partial_sums[static_cast<size_t>(b) * experts + e] : 0.0f;
+        count += e < experts ? a.partial_counts[static_cast<size_t>(b) * (experts + 1u) + e] : 0u;
+    }
+    sums[warp][lane] = sum;
+    routes[warp][lane] = count;
+    __syncthreads();
+    LossParts parts = {counted_shared, 0.0f};
+    if (warp == 0u)
+    {
+        if (e < experts)
+        {
+            float total = 0.0f;
+            uint32_t all = 0;
+            for (uint32_t w = 0; w < 32u; ++w)
+            {
+                total += sums[w][lane];
+                all += routes[w][lane];
+            }
+            store_expert(a, parts, e, total, all);
+        }
+        const float weighted = warp_sum(parts.weighted);
+        if (lane == 0)
+        {
+            a.partial_loss[blockIdx.x] = weighted;
+            __threadfence();
+            last_shared = atomicAdd(a.reduce_done, 1u) == gridDim.x - 1u ? 1u : 0u;
+        }
+    }
+    __syncthreads();
+    if (last_shared == 0u)
+        return;
+    __threadfence();
+    parts.weighted = threadIdx.x < gridDim.x ? a.partial_loss[threadIdx.x] : 0.0f;
+    if (threadIdx.x == 0)
+        *a.reduce_done = 0u;
+    store_loss(a, parts);
+}
+
+// ---- backward -----------------------------------------------------------------------------
+
+template<int kFunction, int kPer>
+__global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const BalanceArgs a, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient)
+{
+    extern __shared__ __align__(16) unsigned char shared_raw[];
+    const uint32_t experts = a.expert_count;
+    const uint32_t warps = blockDim.x / 32u;
+    float* shares = reinterpret_cast<float*>(shared_raw); // [experts]: g, without a constant that does not matter
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     __shared__ unsigned long long routes_shared;
     if (threadIdx.x == 0)
         routes_shared = 0ull;
+    wait_for_previous_kernel();
     __syncthreads();
     unsigned long long mine = 0;
     for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
         mine += expert_tokens[e];
-    atomicAdd(&routes_shared, mine);
+    if (mine != 0ull)
+        atomicAdd(&routes_shared, mine);
     __syncthreads();
     const double counted = static_cast<double>(max(expert_tokens[experts], 1u));
     const double unit = static_cast<double>(a.coefficient) * (loss_gradient != nullptr ? static_cast<double>(*loss_gradient) : 1.0) / (static_cast<double>(a.top_k) * counted * counted);
     for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
         shares[e] = static_cast<float>(unit * static_cast<double>(static_cast<long long>(experts) * static_cast<long long>(expert_tokens[e]) - static_cast<long long>(routes_shared)));
     __syncthreads();
-    for (uint64_t token = static_cast<uint64_t>(blockIdx.x) * warps + warp; token < a.token_count; token += static_cast<uint64_t>(gridDim.x) * warps)
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * warps + warp, stride = static_cast<uint64_t>(gridDim.x) * warps;
+    if constexpr (kPer > 0)
     {
-        float* target = gradient + token * experts;
-        if (a.token_mask != nullptr && a.token_mask[token] == 0)
+        float share[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            share[i] = lane + 32u * i < experts ? shares[lane + 32u * i] : 0.0f;
+        for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            for (uint32_t e = lane; e < experts; e += 32u)
-                target[e] = 0.0f;
-            continue;
+            float* target = gradient + token * experts;
+            float x[kPer], slope[kPer];
+            if (!counts(a, token))
+            {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (lane + 32u * i < experts)
+                        target[lane + 32u * i] = 0.0f;
+                continue;
+            }
+            const float* logits = a.logits + token * experts;
+            float peak = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+            {
+                const uint32_t e = lane + 32u * i;
+                x[i] = e < experts ? logits[e] : 0.0f;
+                if (e < experts)
+                    peak = fmaxf(peak, x[i]);
+            }
+            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
+                peak = warp_max(peak);
+            float total = 0.0f, mean = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+            {
+                float score;
+                score_of<kFunction, true>(x[i], peak, score, slope[i]);
+                if (lane + 32u * i >= experts)
+                    score = 0.0f;
+                total += score;
+                mean = fmaf(share[i], score, mean);
+            }
+#pragma unroll
+            for (int offset = 16; offset > 0; offset >>= 1) // two sums side by side
+            {
+                total += __shfl_xor_sync(kFullMask, total, offset);
+                mean += __shfl_xor_sync(kFullMask, mean, offset);
+            }
+            const float factor = factor_of(total);
+            mean *= factor;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (lane + 32u * i < experts)
+                    target[lane + 32u * i] = factor == 0.0f ? 0.0f : slope[i] * factor * (share[i] - mean);
         }
-        const float* logits = a.logits + token * experts;
-        const float factor = score_row(logits, experts, a.score_function, row);
-        float mean = 0.0f;
-        for (uint32_t e = lane; e < experts; e += 32u)
-            mean += shares[e] * (row[e] * factor);
-        mean = warp_sum(mean);
-        for (uint32_t e = lane; e < experts; e += 32u)
+    }
+    else
+    {
+        for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            const float slope = a.score_function == MOE_ROUTER_SOFTMAX ? row[e] : score_slope(logits[e], row[e], a.score_function);
-            target[e] = factor == 0.0f ? 0.0f : slope * factor * (shares[e] - mean);
+            float* target = gradient + token * experts;
+            if (!counts(a, token))
+            {
+                for (uint32_t e = lane; e < experts; e += 32u)
+                    target[e] = 0.0f;
+                continue;
+            }
+            const float* logits = a.logits + token * experts;
+            float peak = -INFINITY;
+            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
+            {
+                for (uint32_t e = lane; e < experts; e += 32u)
+                    peak = fmaxf(peak, logits[e]);
+                peak = warp_max(peak);
+            }
+            float total = 0.0f, mean = 0.0f;
+            for (uint32_t e = lane; e < experts; e += 32u)
+            {
+                float score, slope;
+                score_of<kFunction, false>(logits[e], peak, score, slope);
+                total += score;
+                mean = fmaf(shares[e], score, mean);
+            }
+            const float factor = factor_of(warp_sum(total));
+            mean = warp_sum(mean) * factor;
+            for (uint32_t e = lane; e < experts; e += 32u)
+            {
+                float score, slope;
+                score_of<kFunction, true>(logits[e], peak, score, slope);
+                target[e] = factor == 0.0f ? 0.0f : slope * factor * (shares[e] - mean);
+            }
         }
     }
 }
 
+// ---- launches -----------------------------------------------------------------------------
+
 uint32_t warps_for(uint32_t experts)
 {
-    return experts <= 1024u ? kBalanceWarps : kBalanceWarps / 2;
+    return experts <= kRegisterExperts ? kBalanceWarps : kWideWarps;
+}
+uint32_t blocks_for(uint32_t token_count, uint32_t experts, uint32_t most)
+{
+    const uint32_t wanted = (token_count + warps_for(experts) - 1u) / warps_for(experts);
+    return wanted < most ? wanted : most;
+}
+
+template<int kFunction, int kPer>
+cudaError_t launch_forward(const BalanceArgs& a, cudaStream_t stream)
+{
+    const uint32_t warps = warps_for(a.expert_count);
+    // one block alone (and no second launch) for up to four tokens a warp
+    const uint32_t blocks = a.token_count <= 4u * warps ? 1u : blocks_for(a.token_count, a.expert_count, MOE_BALANCE_MAX_BLOCKS);
+    const size_t shared_bytes = sizeof(uint32_t) * (2u * a.expert_count + 1u) + sizeof(float) * (kPer > 0 ? 1u : 2u) * warps * a.expert_count;
+    static SharedOptIn opt_in;
+    if (shared_bytes > 48u * 1024u)
+        if (cudaError_t status = opt_in_shared(opt_in, balance_partial_kernel<kFunction, kPer>, shared_bytes))
+            return status;
+    if (cudaError_t status = launch_following(balance_partial_kernel<kFunction, kPer>, blocks, warps * 32u, shared_bytes, stream, a))
+        return status;
+    return blocks == 1u ? cudaSuccess : launch_following(balance_reduce_kernel, (a.expert_count + 31u) / 32u, 1024u, 0, stream, a, blocks);
+}
+
+struct BackwardArgs
+{
+    const uint32_t* expert_tokens;
+    const float* loss_gradient;
+    float* gradient;
+};
+template<int kFunction, int kPer>
+cudaError_t launch_backward(const BalanceArgs& a, const BackwardArgs& b, cudaStream_t stream)
+{
+    const uint32_t warps = warps_for(a.expert_count);
+    return launch_following(balance_backward_kernel<kFunction, kPer>, blocks_for(a.token_count, a.expert_count, 148u * 4u), warps * 32u, sizeof(float) * a.expert_count, stream, a,
+                            b.expert_tokens, b.loss_gradient, b.gradient);
+}
+
+template<int kFunction, int kPer>
+cudaError_t launch(const BalanceArgs& a, const BackwardArgs* b, cudaStream_t stream)
+{
+    return b != nullptr ? launch_backward<kFunction, kPer>(a, *b, stream) : launch_forward<kFunction, kPer>(a, stream);
+}
+template<int kFunction>
+cudaError_t launch_for_experts(const BalanceArgs& a, const BackwardArgs* b, cudaStream_t stream)
+{
+    if (a.expert_count <= 64u)
+        return launch<kFunction, 2>(a, b, stream);
+    if (a.expert_count <= 128u)
+        return launch<kFunction, 4>(a, b, stream);
+    if (a.expert_count <= 256u)
+        return launch<kFunction, 8>(a, b, stream);
+    if (a.expert_count <= 512u)
+        return launch<kFunction, 16>(a, b, stream);
+    if (a.expert_count <= kRegisterExperts)
+        return launch<kFunction, 32>(a, b, stream);
+    return launch<kFunction, 0>(a, b, stream);
+}
+cudaError_t launch_balance(const BalanceArgs& a, const BackwardArgs* b, cudaStream_t stream)
+{
+    switch (a.score_function)
+    {
+    case MOE_ROUTER_SOFTMAX: return launch_for_experts<MOE_ROUTER_SOFTMAX>(a, b, stream);
+    case MOE_ROUTER_SIGMOID: return launch_for_experts<MOE_ROUTER_SIGMOID>(a, b, stream);
+    default: return launch_for_experts<MOE_ROUTER_SQRT_SOFTPLUS>(a, b, stream);
+    }
 }
 
 } // namespace
 
-uint32_t balance_blocks(uint32_t token_count, uint32_t experts)
-{
-    const uint32_t wanted = (token_count + warps_for(experts) - 1u) / warps_for(experts);
-    return wanted < MOE_BALANCE_MAX_BLOCKS ? (wanted > 0u ? wanted : 1u) : MOE_BALANCE_MAX_BLOCKS;
-}
-
 cudaError_t launch_balance_loss(const BalanceArgs& args, cudaStream_t stream)
 {
-    const uint32_t blocks = balance_blocks(args.token_count, args.expert_count);
-    const uint32_t warps = warps_for(args.expert_count);
-    const size_t shared_bytes = sizeof(float) * (2u * warps + 2u) * args.expert_count + sizeof(uint32_t);
-    static SharedOptIn opt_in;
-    if (shared_bytes > 48u * 1024u)
-        if (cudaError_t status = opt_in_shared(opt_in, balance_partial_kernel, shared_bytes))
-            return status;
-    if (cudaError_t status = launch_following(balance_partial_kernel, blocks, warps * 32u, shared_bytes, stream, args))
-        return status;
-    return launch_following(balance_reduce_kernel, 1u, 1024u, 0, stream, args, blocks);
+    return launch_balance(args, nullptr, stream);
 }
 
 cudaError_t launch_balance_loss_backward(const BalanceArgs& args, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient, cudaStream_t stream)
 {
-    const uint32_t blocks = balance_blocks(args.token_count, args.expert_count);
-    const uint32_t warps = warps_for(args.expert_count);
-    const size_t shared_bytes = sizeof(float) * (warps + 1u) * args.expert_count;
-    static SharedOptIn opt_in;
-    if (shared_bytes > 48u * 1024u)
-        if (cudaError_t status = opt_in_shared(opt_in, balance_backward_kernel, shared_bytes))
-            return status;
-    return launch_following(balance_backward_kernel, blocks, warps * 32u, shared_bytes, stream, args, expert_tokens, loss_gradient, gradient);
+    const BackwardArgs backward = {expert_tokens, loss_gradient, gradient};
+    return launch_balance(args, &backward, stream);
 }
 
 } // namespace moe

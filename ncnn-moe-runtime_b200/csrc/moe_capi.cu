@@ -74,8 +74,11 @@ struct moe_sampler
     int32_t* gather_status = nullptr;        // one word: set when moe_regroup_gather met a token index out of range
     // expert products and balance
     uint32_t* expert_flags = nullptr;  // one word: MOE_EXPERT_FLAG_* met since the last check
+    uint8_t* quantize_once = nullptr;  // rows that are quantised once and copied to their routes
+    size_t quantize_once_capacity = 0;
     uint32_t* combine_slots = nullptr; // zeros between calls
     size_t combine_slots_capacity = 0;
+    uint32_t* balance_tail = nullptr;  // a counter, 0 between calls, and MOE_EXPERT_MAX_EXPERTS / 32 parts of a loss
     float* balance_sums = nullptr;
     uint32_t* balance_counts = nullptr;
     size_t balance_sums_capacity = 0;
@@ -310,6 +313,7 @@ int moe_sampler_create(int device, uint32_t max_rows, uint32_t max_vocab, moe_sa
     allocate(reinterpret_cast<void**>(&sampler->gather_status), sizeof(int32_t));
     allocate(reinterpret_cast<void**>(&sampler->router_status_dev), sizeof(int32_t));
     allocate(reinterpret_cast<void**>(&sampler->expert_flags), sizeof(uint32_t));
+    allocate(reinterpret_cast<void**>(&sampler->balance_tail), sizeof(uint32_t) * (1u + MOE_EXPERT_MAX_EXPERTS / 32u));
     if (status == cudaSuccess)
         status = cudaMemset(counters, 0, 8 * sizeof(uint32_t));
     if (status == cudaSuccess)
@@ -322,6 +326,8 @@ int moe_sampler_create(int device, uint32_t max_rows, uint32_t max_vocab, moe_sa
         status = cudaMemset(sampler->gather_status, 0, sizeof(int32_t));
     if (status == cudaSuccess)
         status = cudaMemset(sampler->expert_flags, 0, sizeof(uint32_t));
+    if (status == cudaSuccess)
+        status = cudaMemset(sampler->balance_tail, 0, sizeof(uint32_t));
     if (status == cudaSuccess)
         status = cudaStreamCreateWithFlags(&sampler->stream, cudaStreamNonBlocking);
     if (status == cudaSuccess)
@@ -355,8 +361,8 @@ void moe_sampler_destroy(moe_sampler* sampler)
                         sampler->router_offsets_dev, sampler->router_token_dev, sampler->router_rank_dev, sampler->router_weight_dev,
                         sampler->router_status_dev, sampler->spec_kept_token, sampler->spec_kept_probability, sampler->spec_kept_count,
                         sampler->spec_token, sampler->spec_probability, sampler->spec_flags, sampler->spec_status, sampler->spec_dense,
-                        sampler->spec_residual_token, sampler->spec_residual_value, sampler->expert_flags, sampler->combine_slots,
-                        sampler->balance_sums, sampler->balance_counts};
+                        sampler->spec_residual_token, sampler->spec_residual_value, sampler->expert_flags, sampler->quantize_once, sampler->combine_slots,
+                        sampler->balance_tail, sampler->balance_sums, sampler->balance_counts};
     for (void* pointer : pointers)
         if (pointer != nullptr)
             cudaFree(pointer);
@@ -1062,7 +1068,15 @@ int moe_quantize_rows(moe_sampler* sampler, void* stream_handle, const void* sou
     if (args.rows == 0 || columns == 0)
         return MOE_STATUS_OK;
     DeviceGuard guard(sampler->device);
-    MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, static_cast<cudaStream_t>(stream_handle)));
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+    const size_t once = quantize_once_bytes(args);
+    if (once > sampler->quantize_once_capacity)
+    {
+        // earlier calls on this stream may still use the scratch that is replaced here
+        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
+        MOE_CUDA_CHECK(sampler, grow(sampler->quantize_once, sampler->quantize_once_capacity, once));
+    }
+    MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, once > 0 ? sampler->quantize_once : nullptr, stream));
     return MOE_STATUS_OK;
 }
 
@@ -1095,7 +1109,7 @@ int moe_combine_routes(moe_sampler* sampler, void* stream_handle, const void* ro
         return MOE_STATUS_OK;
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     DeviceGuard guard(sampler->device);
-    const size_t slots = static_cast<size_t>(token_count) * top_k;
+    const size_t slots = combine_few(route_count, token_count, top_k) ? 0u : static_cast<size_t>(token_count) * top_k;
     if (slots > sampler->combine_slots_capacity)
     {
         // earlier calls on this stream may still use the scratch that is replaced here
@@ -1130,7 +1144,8 @@ int moe_balance_loss(moe_sampler* sampler, void* stream_handle, const float* rou
     if (precheck != 0)
         return fail(sampler, moe_router_status_error_code(precheck), moe_router_status_message(precheck));
     BalanceArgs args = {router_logits, token_count, options->expert_count, options->top_k, options->score_function, coefficient, token_mask,
-                        expert_offsets, route_token, expert_tokens, expert_probability, loss, nullptr, nullptr, sampler->expert_flags};
+                        expert_offsets, route_token, expert_tokens, expert_probability, loss, nullptr, nullptr,
+                        reinterpret_cast<float*>(sampler->balance_tail + 1), sampler->balance_tail, sampler->expert_flags};
     if (const char* text = check_balance(args))
         return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
     if (router_logits == nullptr || expert_offsets == nullptr || route_token == nullptr || expert_tokens == nullptr || expert_probability == nullptr ||

@@ -3,6 +3,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "moe_common.cuh"
 #include "moe_internal.h"
 
@@ -11,19 +13,6 @@ namespace moe {
 namespace {
 
 // ---- eight values of a row as floats ----------------------------------------------
-
-template<typename T>
-__device__ __forceinline__ float widen(T value);
-template<>
-__device__ __forceinline__ float widen<float>(float value)
-{
-    return value;
-}
-template<>
-__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 value)
-{
-    return __bfloat162float(value);
-}
 
 // Eight values as they lie in memory: one 16-byte vector of bf16, two of fp32.
 template<typename T>
@@ -206,6 +195,47 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
     }
 }
 
+// Rows that were quantised once, copied to every route that names them: a byte a value from L2 and to HBM.  A warp copies a row,
+// 4 KiB in flight; the scales, which lie block by block, follow in a loop of their own.
+constexpr int kSpreadThreads = 256;
+__global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const QuantizeArgs a, const uint8_t* values, const float* scales)
+{
+    wait_for_previous_kernel();
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t warps = gridDim.x * (kSpreadThreads / 32);
+    const uint32_t vectors = a.columns / 16u;
+    for (uint32_t route = blockIdx.x * (kSpreadThreads / 32) + (threadIdx.x >> 5); route < a.rows; route += warps)
+    {
+        const uint32_t token = a.route_token[route];
+        const bool valid = token < a.source_rows;
+        if (!valid && lane == 0)
+            atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
+        const uint4* source = reinterpret_cast<const uint4*>(values + static_cast<size_t>(valid ? token : 0u) * a.columns);
+        uint4* target = reinterpret_cast<uint4*>(a.values + static_cast<size_t>(route) * a.columns);
+        for (uint32_t first = lane; first < vectors; first += 256u)
+        {
+            uint4 part[8];
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                part[i] = valid && first + 32u * i < vectors ? source[first + 32u * i] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (first + 32u * i < vectors)
+                    target[first + 32u * i] = part[i];
+        }
+    }
+    const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
+    const uint32_t threads = gridDim.x * kSpreadThreads;
+    for (uint32_t route = blockIdx.x * kSpreadThreads + threadIdx.x; route < a.rows; route += threads)
+    {
+        const uint32_t token = a.route_token[route];
+        const bool valid = token < a.source_rows;
+#pragma unroll 8
+        for (uint32_t block = 0; block < blocks; ++block)
+            a.scales[static_cast<size_t>(block) * a.rows + route] = valid ? scales[static_cast<size_t>(block) * a.source_rows + token] : 0.0f;
+    }
+}
+
 template<typename T>
 cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t stream)
 {
@@ -221,10 +251,16 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
 
 // ---- combine --------------------------------------------------------------------------
 //
-// A token's routes lie in the blocks of its experts.  The first kernel notes for every (token, rank) the route that holds
-// it, the second sums a token's rows with one CTA, ranks ascending, and leaves the notes at zero for the next call.
+// A token's routes lie in the blocks of its experts.  HBM bound: every routed row is read once, every token written once.
+// Many routes: one kernel notes for every (token, rank) the route that holds it, the next sums a token's rows with one CTA and
+// leaves the notes at zero for the next call.  Few routes: each CTA looks through all of them for those of its token, which
+// is cheaper than a second launch.  Either way a CTA first has the list of its token's routes and weights, ranks ascending, in
+// shared memory; then a thread adds 16 bytes of up to eight rows at a time.
 
 constexpr int kCombineThreads = 256;
+constexpr uint32_t kCombineFew = 4096;     // routes that every CTA looks through itself
+constexpr uint32_t kCombineFewTokens = 2048;
+constexpr uint32_t kCombineFewRanks = 64;
 
 __global__ void __launch_bounds__(256) combine_slots_kernel(const CombineArgs a)
 {
@@ -239,62 +275,214 @@ __global__ void __launch_bounds__(256) combine_slots_kernel(const CombineArgs a)
     }
 }
 
-template<typename T>
-__device__ __forceinline__ void store_narrow(T* target, float value);
-template<>
-__device__ __forceinline__ void store_narrow<float>(float* target, float value)
+__device__ __forceinline__ void narrow(float* target, const float (&x)[4])
 {
-    *target = value;
+    *reinterpret_cast<float4*>(target) = make_float4(x[0], x[1], x[2], x[3]);
 }
-template<>
-__device__ __forceinline__ void store_narrow<__nv_bfloat16>(__nv_bfloat16* target, float value)
+__device__ __forceinline__ void narrow(__nv_bfloat16* target, const float (&x)[8])
 {
-    *target = __float2bfloat16_rn(value);
+    uint32_t words[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const __nv_bfloat162 pair = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        memcpy(&words[i], &pair, 4);
+    }
+    *reinterpret_cast<uint4*>(target) = make_uint4(words[0], words[1], words[2], words[3]);
+}
+__device__ __forceinline__ void narrow(float* target, const float (&x)[1])
+{
+    *target = x[0];
+}
+__device__ __forceinline__ void narrow(__nv_bfloat16* target, const float (&x)[1])
+{
+    *target = __float2bfloat16_rn(x[0]);
+}
+// sum += weight * row
+__device__ __forceinline__ void add_weighted(float (&sum)[4], const uint4& row, float weight)
+{
+    sum[0] = fmaf(weight, __uint_as_float(row.x), sum[0]);
+    sum[1] = fmaf(weight, __uint_as_float(row.y), sum[1]);
+    sum[2] = fmaf(weight, __uint_as_float(row.z), sum[2]);
+    sum[3] = fmaf(weight, __uint_as_float(row.w), sum[3]);
+}
+__device__ __forceinline__ void add_weighted(float (&sum)[8], const uint4& row, float weight)
+{
+    const uint32_t words[4] = {row.x, row.y, row.z, row.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        sum[2 * i] = fmaf(weight, __uint_as_float(words[i] << 16), sum[2 * i]);
+        sum[2 * i + 1] = fmaf(weight, __uint_as_float(words[i] & 0xFFFF0000u), sum[2 * i + 1]);
+    }
+}
+__device__ __forceinline__ void add_weighted(float (&sum)[1], float row, float weight)
+{
+    sum[0] = fmaf(weight, row, sum[0]);
+}
+__device__ __forceinline__ void add_weighted(float (&sum)[1], __nv_bfloat16 row, float weight)
+{
+    sum[0] = fmaf(weight, __bfloat162float(row), sum[0]);
 }
 
-template<typename T>
+// Columns [begin, end) of a token: base plus the listed rows, in their order.  kWidth values of a thread at a time: 16 bytes, or
+// one where a row does not start at a multiple of 16.
+template<typename T, bool kVector>
+__device__ __forceinline__ void sum_token(const CombineArgs& a, uint32_t token, const uint2* list, uint32_t count, uint32_t begin, uint32_t end)
+{
+    using Load = std::conditional_t<kVector, uint4, T>;
+    constexpr uint32_t kWidth = kVector ? 16u / sizeof(T) : 1u;
+    constexpr uint32_t kRows = 8; // in flight
+    const T* rows = static_cast<const T*>(a.route_rows);
+    for (uint32_t column = begin + threadIdx.x * kWidth; column < end; column += kCombineThreads * kWidth)
+    {
+        float sum[kWidth] = {};
+        if (a.base != nullptr)
+            add_weighted(sum, *reinterpret_cast<const Load*>(static_cast<const T*>(a.base) + static_cast<size_t>(token) * a.columns + column), 1.0f);
+        for (uint32_t first = 0; first < count; first += kRows)
+        {
+            Load part[kRows];
+#pragma unroll
+            for (uint32_t i = 0; i < kRows; ++i)
+                if (first + i < count)
+                    part[i] = *reinterpret_cast<const Load*>(rows + static_cast<size_t>(list[first + i].x) * a.row_stride + column);
+#pragma unroll
+            for (uint32_t i = 0; i < kRows; ++i)
+                if (first + i < count)
+                    add_weighted(sum, part[i], __uint_as_float(list[first + i].y));
+        }
+        narrow(static_cast<T*>(a.out) + static_cast<size_t>(token) * a.columns + column, sum);
+    }
+}
+
+// Packs the routes noted in slots[0 .. top_k) (0: none), which may be global or shared memory, with their weights.  One warp;
+// returns their number.
+__device__ __forceinline__ uint32_t list_routes(const CombineArgs& a, const uint32_t* slots, uint2* list)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t count = 0;
+    for (uint32_t first = 0; first < a.top_k; first += 32u)
+    {
+        const uint32_t slot = first + lane < a.top_k ? slots[first + lane] : 0u;
+        const unsigned taken = __ballot_sync(kFullMask, slot != 0u);
+        if (slot != 0u)
+            list[count + __popc(taken & ((1u << lane) - 1u))] = make_uint2(slot - 1u, __float_as_uint(a.route_weight[slot - 1u]));
+        count += __popc(taken);
+    }
+    return count;
+}
+
+template<typename T, bool kVector>
 __global__ void __launch_bounds__(kCombineThreads) combine_routes_kernel(const CombineArgs a)
 {
+    extern __shared__ __align__(16) unsigned char shared_raw[];
+    uint2* list = reinterpret_cast<uint2*>(shared_raw); // [top_k]
+    __shared__ uint32_t count_shared;
     wait_for_previous_kernel();
     for (uint32_t token = blockIdx.x; token < a.token_count; token += gridDim.x)
     {
         uint32_t* slots = a.slots + static_cast<size_t>(token) * a.top_k;
-        for (uint32_t column = threadIdx.x; column < a.columns; column += kCombineThreads)
+        if (threadIdx.x < 32u)
         {
-            float sum = a.base != nullptr ? widen(static_cast<const T*>(a.base)[static_cast<size_t>(token) * a.columns + column]) : 0.0f;
-            for (uint32_t rank = 0; rank < a.top_k; ++rank)
-            {
-                const uint32_t slot = slots[rank];
-                if (slot != 0u)
-                    sum = fmaf(a.route_weight[slot - 1u], widen(static_cast<const T*>(a.route_rows)[static_cast<size_t>(slot - 1u) * a.row_stride + column]), sum);
-            }
-            store_narrow(static_cast<T*>(a.out) + static_cast<size_t>(token) * a.columns + column, sum);
+            const uint32_t count = list_routes(a, slots, list);
+            if (threadIdx.x == 0)
+                count_shared = count;
+            __syncwarp();
+            for (uint32_t rank = threadIdx.x; rank < a.top_k; rank += 32u)
+                slots[rank] = 0u;
         }
         __syncthreads();
-        for (uint32_t rank = threadIdx.x; rank < a.top_k; rank += kCombineThreads)
-            slots[rank] = 0u;
+        sum_token<T, kVector>(a, token, list, count_shared, 0u, a.columns);
+        __syncthreads();
     }
+}
+
+// A CTA for `piece` columns of a token; it looks through all routes.
+template<typename T, bool kVector>
+__global__ void __launch_bounds__(kCombineThreads) combine_few_kernel(const CombineArgs a, uint32_t pieces, uint32_t piece)
+{
+    __shared__ uint32_t slots[kCombineFewRanks];
+    __shared__ uint2 list[kCombineFewRanks];
+    __shared__ uint32_t count_shared;
+    wait_for_previous_kernel();
+    const uint32_t token = blockIdx.x / pieces;
+    const uint32_t begin = (blockIdx.x - token * pieces) * piece;
+    for (uint32_t rank = threadIdx.x; rank < a.top_k; rank += kCombineThreads)
+        slots[rank] = 0u;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < a.route_count; i += kCombineThreads)
+    {
+        const uint32_t of = a.route_token[i], rank = a.route_rank[i];
+        if (of == token && rank < a.top_k)
+            atomicMax(&slots[rank], i + 1u);
+        if (blockIdx.x == 0 && (of >= a.token_count || rank >= a.top_k))
+            atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32u)
+    {
+        const uint32_t count = list_routes(a, slots, list);
+        if (threadIdx.x == 0)
+            count_shared = count;
+    }
+    __syncthreads();
+    sum_token<T, kVector>(a, token, list, count_shared, begin, min(a.columns, begin + piece));
+}
+
+template<typename T>
+cudaError_t launch_combine(const CombineArgs& a, cudaStream_t stream)
+{
+    constexpr uint32_t kWidth = 16u / sizeof(T);
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(a.route_rows) | reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out);
+    const bool vector = a.columns % kWidth == 0u && a.row_stride % kWidth == 0u && bases % 16u == 0u;
+    if (combine_few(a.route_count, a.token_count, a.top_k))
+    {
+        // pieces of what a CTA's threads take at once, fewer when that gives more CTAs than are resident
+        const uint32_t step = kCombineThreads * (vector ? kWidth : 1u);
+        uint32_t pieces = (a.columns + step - 1u) / step;
+        while (pieces > 1u && static_cast<uint64_t>(pieces) * a.token_count > 148u * 8u)
+            pieces = (pieces + 1u) / 2u;
+        const uint32_t piece = ((a.columns + pieces - 1u) / pieces + step - 1u) / step * step;
+        auto kernel = vector ? combine_few_kernel<T, true> : combine_few_kernel<T, false>;
+        return launch_following(kernel, pieces * a.token_count, kCombineThreads, 0, stream, a, pieces, piece);
+    }
+    const uint32_t blocks = (a.route_count + 255u) / 256u;
+    if (cudaError_t status = launch_following(combine_slots_kernel, blocks < 592u ? blocks : 592u, 256u, 0, stream, a))
+        return status;
+    auto kernel = vector ? combine_routes_kernel<T, true> : combine_routes_kernel<T, false>;
+    return launch_following(kernel, a.token_count < 148u * 8u ? a.token_count : 148u * 8u, kCombineThreads, sizeof(uint2) * a.top_k, stream, a);
 }
 
 } // namespace
 
-cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, cudaStream_t stream)
+cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, uint8_t* once, cudaStream_t stream)
 {
     const bool gate = activation == MOE_ACTIVATION_SILU_GATE;
+    if (once != nullptr)
+    {
+        // every source row once, then a copy for each route
+        QuantizeArgs rows = args;
+        rows.route_token = nullptr;
+        rows.rows = args.source_rows;
+        rows.values = once;
+        rows.scales = reinterpret_cast<float*>(once + (static_cast<size_t>(args.source_rows) * args.columns + 15u) / 16u * 16u);
+        const cudaError_t status = dtype == MOE_DTYPE_F32 ? launch_quantize<float>(rows, gate, stream) : launch_quantize<__nv_bfloat16>(rows, gate, stream);
+        if (status != cudaSuccess)
+            return status;
+        const uint32_t blocks = (args.rows + kSpreadThreads / 32 - 1) / (kSpreadThreads / 32);
+        return launch_following(spread_rows_kernel, blocks < 148u * 8u ? blocks : 148u * 8u, kSpreadThreads, 0, stream, args, rows.values, rows.scales);
+    }
     return dtype == MOE_DTYPE_F32 ? launch_quantize<float>(args, gate, stream) : launch_quantize<__nv_bfloat16>(args, gate, stream);
+}
+
+bool combine_few(uint32_t route_count, uint32_t token_count, uint32_t top_k)
+{
+    return route_count <= kCombineFew && token_count <= kCombineFewTokens && top_k <= kCombineFewRanks;
 }
 
 cudaError_t launch_combine_routes(const CombineArgs& args, int dtype, cudaStream_t stream)
 {
-    if (args.route_count > 0)
-    {
-        const uint64_t blocks = (static_cast<uint64_t>(args.route_count) + 255u) / 256u;
-        if (cudaError_t status = launch_following(combine_slots_kernel, static_cast<uint32_t>(blocks < 592u ? blocks : 592u), 256u, 0, stream, args))
-            return status;
-    }
-    const uint32_t grid = args.token_count < 148u * 8u ? args.token_count : 148u * 8u;
-    return dtype == MOE_DTYPE_F32 ? launch_following(combine_routes_kernel<float>, grid, kCombineThreads, 0, stream, args)
-                                  : launch_following(combine_routes_kernel<__nv_bfloat16>, grid, kCombineThreads, 0, stream, args);
+    return dtype == MOE_DTYPE_F32 ? launch_combine<float>(args, stream) : launch_combine<__nv_bfloat16>(args, stream);
 }
 
 } // namespace moe

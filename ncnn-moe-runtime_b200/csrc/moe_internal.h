@@ -17,8 +17,8 @@
 #define MOE_SPECULATIVE_SHORT_LIST 1024u
 // entries of the router's [expert][block] count table (expert_count * blocks of the select kernel never exceeds it)
 #define MOE_ROUTER_BLOCK_TABLE_ENTRIES 262144u
-// blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): two per SM
-#define MOE_BALANCE_MAX_BLOCKS 296u
+// blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): four per SM
+#define MOE_BALANCE_MAX_BLOCKS 592u
 
 namespace moe {
 
@@ -363,9 +363,26 @@ struct BalanceArgs
     float* loss;
     float* partial_sums;      // [MOE_BALANCE_MAX_BLOCKS][expert_count]
     uint32_t* partial_counts; // [MOE_BALANCE_MAX_BLOCKS][expert_count + 1]
+    float* partial_loss;      // [MOE_EXPERT_MAX_EXPERTS / 32]
+    uint32_t* reduce_done;    // one word, 0 between calls
     uint32_t* flags;
 };
-cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, cudaStream_t stream);
+// once: scratch of quantize_once_bytes for rows that are quantised once and then copied to their routes, or null
+cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, uint8_t* once, cudaStream_t stream);
+// Scratch for quantising each source row once, 0 where every route quantises its own row.  Dividing is what a call is bound by
+// (12 instructions a value), so rows with two routes or more on average gain: 4096 rows x 4096 to 32768 routes 87 us route by
+// route, %ONCE% in two passes.  The quantised rows have to stay in L2 between the passes, and are copied in 16-byte vectors; small
+// calls gain nothing from a second launch.
+inline size_t quantize_once_bytes(const QuantizeArgs& a)
+{
+    const size_t values = (static_cast<size_t>(a.source_rows) * a.columns + 15u) / 16u * 16u;
+    const size_t bytes = values + sizeof(float) * a.source_rows * ((static_cast<size_t>(a.columns) + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK);
+    const bool worth = a.route_token != nullptr && a.rows / 2u >= a.source_rows && static_cast<uint64_t>(a.rows) * a.columns >= (1ull << 22);
+    const bool fits = a.columns % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 16u == 0u && a.source_rows > 0u && bytes <= (48ull << 20);
+    return worth && fits ? bytes : 0u;
+}
+// whether a combine needs no slots: each of its CTAs looks through the routes
+bool combine_few(uint32_t route_count, uint32_t token_count, uint32_t top_k);
 cudaError_t launch_expert_product(const ProductArgs& args, int out_dtype, int sm_count, cudaStream_t stream);
 cudaError_t launch_combine_routes(const CombineArgs& args, int dtype, cudaStream_t stream);
 cudaError_t launch_balance_loss(const BalanceArgs& args, cudaStream_t stream);
@@ -438,8 +455,8 @@ inline const char* check_combine(const CombineArgs& a, int dtype)
         return "columns, token_count and route_count must be below 2^31";
     if (a.token_count == 0 || a.columns == 0)
         return nullptr;
-    if (a.top_k == 0 && a.route_count > 0)
-        return "top_k must be positive";
+    if ((a.top_k == 0 && a.route_count > 0) || a.top_k > MOE_EXPERT_MAX_EXPERTS)
+        return "combining needs 0 < top_k <= MOE_EXPERT_MAX_EXPERTS";
     if (a.out == nullptr)
         return "out must not be null";
     if (a.route_count > 0 && (a.route_rows == nullptr || a.route_token == nullptr || a.route_rank == nullptr || a.route_weight == nullptr))

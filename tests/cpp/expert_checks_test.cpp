@@ -90,6 +90,8 @@ int main()
         check("combine no tokens", false, MOE_DTYPE_F32, [](CombineArgs& a) { a.token_count = 0; a.out = nullptr; });
         check("combine no routes", false, MOE_DTYPE_F32, [](CombineArgs& a) { a.route_count = 0; a.route_rows = nullptr; a.route_token = nullptr; });
         check("combine top_k", true, MOE_DTYPE_F32, [](CombineArgs& a) { a.top_k = 0; });
+        check("combine largest top_k", false, MOE_DTYPE_F32, [](CombineArgs& a) { a.top_k = 4096; });
+        check("combine too large top_k", true, MOE_DTYPE_F32, [](CombineArgs& a) { a.top_k = 4097; });
         check("combine null out", true, MOE_DTYPE_F32, [](CombineArgs& a) { a.out = nullptr; });
         check("combine null ranks", true, MOE_DTYPE_F32, [](CombineArgs& a) { a.route_rank = nullptr; });
         check("combine base alignment", true, MOE_DTYPE_F32, [](CombineArgs& a) { a.base = at<void>(66); });

@@ -71,6 +71,26 @@ def test_quantize_gathers(sampler, torch_cuda, dtype, columns):
     assert sampler.expert_check() == 0
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("source_rows,routes,columns", [(300, 4200, 1040), (2500, 5000, 848), (7, 9000, 480), (2500, 4999, 848), (300, 4200, 1032)])
+def test_quantize_gathers_rows_that_are_routed_often(sampler, pkg, torch_cuda, dtype, source_rows, routes, columns):
+    """Two routes a row on average, and 2^22 values: the rows are quantised once and copied (below that, or with columns that are no
+    multiple of 16, they are not)."""
+    torch = torch_cuda
+    x = (randn(torch, 5, source_rows, columns + 8) * 3).to(getattr(torch, dtype))[:, :columns]
+    index = torch.randint(source_rows, (routes,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").int()
+    values, scales = sampler.quantize_rows(x, route_token=index)
+    want_values, want_scales = quantize_reference(torch, x[index.long()])
+    assert torch.equal(scales.cpu(), want_scales) and torch.equal(values.float().cpu(), want_values)
+    assert sampler.expert_check() == 0
+    index[[5, routes - 1]] = torch.tensor([source_rows, -1], dtype=torch.int32, device="cuda")
+    spoiled = sampler.quantize_rows(x, route_token=index)
+    assert sampler.expert_check() == pkg.EXPERT_FLAG_TOKEN_RANGE
+    values.view(torch.uint8)[[5, routes - 1]] = 0
+    scales[:, [5, routes - 1]] = 0
+    assert torch.equal(spoiled[0].view(torch.uint8), values.view(torch.uint8)) and torch.equal(spoiled[1], scales)
+
+
 def test_quantize_strides_alignments_and_sentinels(sampler, torch_cuda):
     """Rows inside a wider matrix, starts that no vector load takes, and nothing written outside the outputs."""
     torch = torch_cuda
@@ -296,7 +316,8 @@ def combine_reference(torch, rows, plan, tokens, base):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("tokens,top_k,columns", [(1, 1, 1), (1, 8, 4096), (32, 4, 2880), (33, 6, 131), (200, 8, 72), (1500, 3, 264), (4, 40, 257), (700, 2, 1030), (3, 1, 8)])
+@pytest.mark.parametrize("tokens,top_k,columns", [(1, 1, 1), (1, 8, 4096), (32, 4, 2880), (33, 6, 131), (200, 8, 72), (1500, 3, 264), (4, 40, 257), (700, 2, 1030), (3, 1, 8), (70, 100, 40), (2100, 1, 9),
+                                                  (600, 8, 512)])
 def test_combine(sampler, torch_cuda, dtype, tokens, top_k, columns):
     """A multiplication per route and a sum of top_k + 1 terms."""
     torch = torch_cuda
