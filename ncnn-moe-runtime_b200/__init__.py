@@ -192,20 +192,34 @@ class BalanceLoss:
 def _value_dtype(tensor, name):
     """DTYPE_* of a float32 or bfloat16 tensor."""
     import torch
-    if tensor.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"{name} must be float32 or bfloat16")
-    return DTYPE_F32 if tensor.dtype == torch.float32 else DTYPE_BF16
+    dtype = tensor.dtype
+    if dtype is torch.float32:
+        return DTYPE_F32
+    if dtype is torch.bfloat16:
+        return DTYPE_BF16
+    raise TypeError(f"{name} must be float32 or bfloat16")
 
 
-def _dense(tensor, name, shape, dtype):
-    """The tensor, which must be contiguous and of this shape and one of these types (None passes)."""
+def _address(tensor, name, shape, dtype, device):
+    """Address of a contiguous tensor of this shape and type on CUDA device `device` (None passes)."""
     if tensor is None:
         return None
-    if tensor.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
-        raise TypeError(f"{name} has dtype {tensor.dtype}")
-    if tuple(tensor.shape) != tuple(shape) or not tensor.is_contiguous():
+    if tensor.dtype is not dtype:
+        raise TypeError(f"{name} has dtype {tensor.dtype}, wanted {dtype}")
+    if tensor.shape != shape or not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous with shape {tuple(shape)}, got {tuple(tensor.shape)}")
-    return tensor
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} must lie on cuda:{device}, the handle's device; got {tensor.device}")
+    return tensor.data_ptr()
+
+
+def _rows_address(tensor, name, device):
+    """Address of a matrix whose columns are adjacent, on CUDA device `device`."""
+    if tensor.dim() != 2 or (tensor.stride(1) != 1 and tensor.shape[0] > 0 and tensor.shape[1] > 1):
+        raise ValueError(f"{name} must be a matrix with adjacent columns")
+    if tensor.get_device() != device:
+        raise ValueError(f"{name} must lie on cuda:{device}, the handle's device; got {tensor.device}")
+    return tensor.data_ptr()
 
 
 class Sampler:
@@ -522,38 +536,36 @@ class Sampler:
         return flag.value != 0
 
     # ---- expert products --------------------------------------------------------------
-    def _place(self, stream, *tensors):
-        """The stream to launch on; every tensor must lie on the handle's device."""
+    def _stream(self, stream):
         import torch
-        for tensor in tensors:
-            if tensor is not None and (not tensor.is_cuda or tensor.device.index != self.device):
-                raise ValueError(f"tensors must lie on cuda:{self.device}, the handle's device; got {tensor.device}")
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream)
+        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else stream
 
     def quantize_rows(self, source, route_token=None, activation=ACTIVATION_NONE, stream=None, out=None):
         """moe_quantize_rows: CUDA float32 / bfloat16 rows [source_rows, columns] (unit column stride; 2 * columns wide with
         ACTIVATION_SILU_GATE) to e4m3.  route_token: int32 [routes] picks the source row of every output row.
         Returns (values float8_e4m3fn [rows, columns], scales float32 [ceil(columns / 128), rows]), written to `out` when given."""
         import torch
+        device = self.device
         dtype = _value_dtype(source, "source")
+        address = _rows_address(source, "source", device)
         source_rows, width = source.shape
-        if source_rows > 1 and width > 0 and source.stride(1) != 1:
-            raise ValueError("the columns of source must be adjacent")
-        if activation == ACTIVATION_SILU_GATE and width % 2:
-            raise ValueError("a gated source has an even number of columns")
-        columns = width // 2 if activation == ACTIVATION_SILU_GATE else width
-        if route_token is not None:
-            _dense(route_token, "route_token", (route_token.numel(),), torch.int32)
+        columns = width
+        if activation == ACTIVATION_SILU_GATE:
+            if width % 2:
+                raise ValueError("a gated source has an even number of columns")
+            columns = width // 2
         rows = source_rows if route_token is None else route_token.numel()
         blocks = (columns + EXPERT_BLOCK - 1) // EXPERT_BLOCK
         if out is None:
             out = (torch.empty((rows, columns), dtype=torch.float8_e4m3fn, device=source.device), torch.empty((blocks, rows), dtype=torch.float32, device=source.device))
-        values, scales = _dense(out[0], "values", (rows, columns), torch.float8_e4m3fn), _dense(out[1], "scales", (blocks, rows), torch.float32)
-        place = self._place(stream, source, route_token, values, scales)
+        values, scales = out
+        routes = _address(route_token, "route_token", (rows,), torch.int32, device)
+        values_address = _address(values, "values", (rows, columns), torch.float8_e4m3fn, device)
+        scales_address = _address(scales, "scales", (blocks, rows), torch.float32, device)
         if rows == 0:
             return values, scales
-        self._check(self._lib.moe_quantize_rows(self._handle, place, _dev_ptr(source), dtype, source_rows, columns, source.stride(0) if source_rows > 1 else width,
-                                                int(activation), _dev_ptr(route_token), rows, _dev_ptr(values), _dev_ptr(scales)))
+        self._check(self._lib.moe_quantize_rows(self._handle, self._stream(stream), address, dtype, source_rows, columns, source.stride(0) if source_rows > 1 else width,
+                                                activation, routes, rows, values_address, scales_address))
         return values, scales
 
     def expert_product(self, values, scales, weights, weight_scales, expert_offsets=None, out_dtype=None, stream=None, out=None):
@@ -562,48 +574,44 @@ class Sampler:
         [experts, ceil(outputs / 128), ceil(columns / 128)]; expert_offsets int32 [experts + 1] (None with one expert).
         Returns [rows, outputs] of out_dtype (bfloat16 unless given), or `out` (unit column stride)."""
         import torch
+        device = self.device
         rows, columns = values.shape
         experts, outputs, _ = weights.shape
         blocks = (columns + EXPERT_BLOCK - 1) // EXPERT_BLOCK
-        _dense(values, "values", (rows, columns), torch.float8_e4m3fn)
-        _dense(scales, "scales", (blocks, rows), torch.float32)
-        _dense(weights, "weights", (experts, outputs, columns), torch.float8_e4m3fn)
-        _dense(weight_scales, "weight_scales", (experts, (outputs + EXPERT_BLOCK - 1) // EXPERT_BLOCK, blocks), torch.float32)
-        _dense(expert_offsets, "expert_offsets", (experts + 1,), torch.int32)
         if out is None:
             out = torch.empty((rows, outputs), dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=values.device)
-        elif tuple(out.shape) != (rows, outputs) or (outputs > 1 and out.stride(1) != 1):
-            raise ValueError(f"out must have shape {(rows, outputs)} and adjacent columns")
-        place = self._place(stream, values, scales, weights, weight_scales, expert_offsets, out)
-        self._check(self._lib.moe_expert_product(self._handle, place, _dev_ptr(values), _dev_ptr(scales), rows, columns, _dev_ptr(weights), _dev_ptr(weight_scales),
-                                                 experts, outputs, _dev_ptr(expert_offsets), _dev_ptr(out), _value_dtype(out, "out"),
-                                                 out.stride(0) if rows > 1 else outputs))
+        elif out.shape != (rows, outputs):
+            raise ValueError(f"out must have shape {(rows, outputs)}, got {tuple(out.shape)}")
+        self._check(self._lib.moe_expert_product(
+            self._handle, self._stream(stream), _address(values, "values", (rows, columns), torch.float8_e4m3fn, device),
+            _address(scales, "scales", (blocks, rows), torch.float32, device), rows, columns,
+            _address(weights, "weights", (experts, outputs, columns), torch.float8_e4m3fn, device),
+            _address(weight_scales, "weight_scales", (experts, (outputs + EXPERT_BLOCK - 1) // EXPERT_BLOCK, blocks), torch.float32, device), experts, outputs,
+            _address(expert_offsets, "expert_offsets", (experts + 1,), torch.int32, device), _rows_address(out, "out", device), _value_dtype(out, "out"),
+            out.stride(0) if rows > 1 else outputs))
         return out
 
     def combine_routes(self, route_rows, route_token, route_rank, route_weight, token_count, top_k, base=None, stream=None, out=None):
         """moe_combine_routes: float32 / bfloat16 rows [routes, columns] (unit column stride) with the plan's route arrays, summed per
         token onto `base` [tokens, columns] (None: zeros).  Returns [tokens, columns], or `out`, which may be `base`."""
         import torch
+        device = self.device
         dtype = _value_dtype(route_rows, "route_rows")
+        address = _rows_address(route_rows, "route_rows", device)
         routes, columns = route_rows.shape
-        if routes > 1 and columns > 1 and route_rows.stride(1) != 1:
-            raise ValueError("the columns of route_rows must be adjacent")
-        for name, tensor, kind in (("route_token", route_token, torch.int32), ("route_rank", route_rank, torch.int32), ("route_weight", route_weight, torch.float32)):
-            _dense(tensor, name, (routes,), kind)
-        _dense(base, "base", (token_count, columns), route_rows.dtype)
         if out is None:
             out = torch.empty((token_count, columns), dtype=route_rows.dtype, device=route_rows.device)
-        _dense(out, "out", (token_count, columns), route_rows.dtype)
-        place = self._place(stream, route_rows, route_token, route_rank, route_weight, base, out)
-        self._check(self._lib.moe_combine_routes(self._handle, place, _dev_ptr(route_rows), dtype, route_rows.stride(0) if routes > 1 else columns, columns,
-                                                 _dev_ptr(route_token), _dev_ptr(route_rank), _dev_ptr(route_weight), routes, int(token_count), int(top_k),
-                                                 _dev_ptr(base), _dev_ptr(out)))
+        self._check(self._lib.moe_combine_routes(
+            self._handle, self._stream(stream), address, dtype, route_rows.stride(0) if routes > 1 else columns, columns,
+            _address(route_token, "route_token", (routes,), torch.int32, device), _address(route_rank, "route_rank", (routes,), torch.int32, device),
+            _address(route_weight, "route_weight", (routes,), torch.float32, device), routes, token_count, top_k,
+            _address(base, "base", (token_count, columns), route_rows.dtype, device), _address(out, "out", (token_count, columns), route_rows.dtype, device)))
         return out
 
     def expert_check(self, stream=None) -> int:
         """moe_expert_check: the EXPERT_FLAG_* bits met since the last check (synchronises)."""
         flags = C.c_uint32(0)
-        self._check(self._lib.moe_expert_check(self._handle, self._place(stream), C.byref(flags)))
+        self._check(self._lib.moe_expert_check(self._handle, self._stream(stream), C.byref(flags)))
         return flags.value
 
     # ---- expert balance ----------------------------------------------------------------
@@ -611,40 +619,38 @@ class Sampler:
                      out=None) -> BalanceLoss:
         """moe_balance_loss: CUDA float32 logits [tokens, experts] and the plan made from them; token_mask bool / uint8 [tokens]."""
         import torch
+        device = self.device
         tokens, experts = router_logits.shape
-        _dense(router_logits, "router_logits", (tokens, experts), torch.float32)
-        _dense(expert_offsets, "expert_offsets", (experts + 1,), torch.int32)
-        _dense(route_token, "route_token", (tokens * top_k,), torch.int32)
-        _dense(token_mask, "token_mask", (tokens,), (torch.bool, torch.uint8))
-        device = router_logits.device
         if out is None:
-            out = BalanceLoss(torch.empty(1, dtype=torch.float32, device=device), torch.empty(experts + 1, dtype=torch.int32, device=device),
-                              torch.empty(experts, dtype=torch.float32, device=device))
-        _dense(out.loss, "loss", (1,), torch.float32)
-        _dense(out.expert_tokens, "expert_tokens", (experts + 1,), torch.int32)
-        _dense(out.expert_probability, "expert_probability", (experts,), torch.float32)
-        options = RouterOptions(experts, int(top_k), int(score_function), 0, 1.0, 0, None, None)
-        place = self._place(stream, router_logits, expert_offsets, route_token, token_mask, out.loss, out.expert_tokens, out.expert_probability)
-        self._check(self._lib.moe_balance_loss(self._handle, place, _dev_ptr(router_logits), tokens, C.byref(options), _dev_ptr(expert_offsets),
-                                               _dev_ptr(route_token), _dev_ptr(token_mask), float(coefficient), _dev_ptr(out.expert_tokens),
-                                               _dev_ptr(out.expert_probability), _dev_ptr(out.loss)))
+            place = router_logits.device
+            out = BalanceLoss(torch.empty(1, dtype=torch.float32, device=place), torch.empty(experts + 1, dtype=torch.int32, device=place),
+                              torch.empty(experts, dtype=torch.float32, device=place))
+        options = RouterOptions(experts, top_k, score_function, 0, 1.0, 0, None, None)
+        self._check(self._lib.moe_balance_loss(
+            self._handle, self._stream(stream), _address(router_logits, "router_logits", (tokens, experts), torch.float32, device), tokens, C.byref(options),
+            _address(expert_offsets, "expert_offsets", (experts + 1,), torch.int32, device), _address(route_token, "route_token", (tokens * top_k,), torch.int32, device),
+            self._mask_address(token_mask, tokens), coefficient, _address(out.expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
+            _address(out.expert_probability, "expert_probability", (experts,), torch.float32, device), _address(out.loss, "loss", (1,), torch.float32, device)))
         return out
+
+    def _mask_address(self, token_mask, tokens):
+        import torch
+        if token_mask is None:
+            return None
+        return _address(token_mask, "token_mask", (tokens,), torch.uint8 if token_mask.dtype is torch.uint8 else torch.bool, self.device)
 
     def balance_loss_backward(self, router_logits, expert_tokens, top_k, score_function=ROUTER_SOFTMAX, token_mask=None, coefficient=1.0, loss_gradient=None,
                               stream=None, out=None):
         """moe_balance_loss_backward: the gradient [tokens, experts] of balance_loss (same arguments, its expert_tokens) times loss_gradient
         (CUDA float32 [1]; None: 1)."""
         import torch
+        device = self.device
         tokens, experts = router_logits.shape
-        _dense(router_logits, "router_logits", (tokens, experts), torch.float32)
-        _dense(expert_tokens, "expert_tokens", (experts + 1,), torch.int32)
-        _dense(token_mask, "token_mask", (tokens,), (torch.bool, torch.uint8))
-        _dense(loss_gradient, "loss_gradient", (1,), torch.float32)
         if out is None:
             out = torch.empty((tokens, experts), dtype=torch.float32, device=router_logits.device)
-        _dense(out, "out", (tokens, experts), torch.float32)
-        options = RouterOptions(experts, int(top_k), int(score_function), 0, 1.0, 0, None, None)
-        place = self._place(stream, router_logits, expert_tokens, token_mask, loss_gradient, out)
-        self._check(self._lib.moe_balance_loss_backward(self._handle, place, _dev_ptr(router_logits), tokens, C.byref(options), _dev_ptr(token_mask),
-                                                        float(coefficient), _dev_ptr(expert_tokens), _dev_ptr(loss_gradient), _dev_ptr(out)))
+        options = RouterOptions(experts, top_k, score_function, 0, 1.0, 0, None, None)
+        self._check(self._lib.moe_balance_loss_backward(
+            self._handle, self._stream(stream), _address(router_logits, "router_logits", (tokens, experts), torch.float32, device), tokens, C.byref(options),
+            self._mask_address(token_mask, tokens), coefficient, _address(expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
+            _address(loss_gradient, "loss_gradient", (1,), torch.float32, device), _address(out, "out", (tokens, experts), torch.float32, device)))
         return out

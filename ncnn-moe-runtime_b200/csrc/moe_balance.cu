@@ -16,10 +16,11 @@ namespace moe {
 
 namespace {
 
-constexpr int kBalanceThreads = 512;
-constexpr int kBalanceWarps = kBalanceThreads / 32;
 constexpr uint32_t kRegisterExperts = 1024; // up to here a lane holds a row's scores in registers
-constexpr int kWideWarps = 4;               // warps of a block for wider rows, which lie in shared memory
+// Threads of a block by the scores a lane holds: two or four blocks to an SM; rows in shared memory (kPer 0) need 32 bytes a
+// warp and expert.
+template<int kPer>
+constexpr int kThreadsFor = kPer == 0 ? 128 : kPer >= 32 ? 256 : 512;
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -82,10 +83,27 @@ __device__ __forceinline__ void score_of(float x, float peak, float& score, floa
     }
 }
 
-__device__ __forceinline__ bool counts(const BalanceArgs& a, uint64_t token)
+__device__ __forceinline__ bool token_counts(const BalanceArgs& a, uint64_t token)
 {
     return a.token_mask == nullptr || a.token_mask[token] != 0;
 }
+// A lane's part of a token's logits: every 32nd.  The next token's are on their way while one is worked on.
+template<int kPer>
+struct LaneRow
+{
+    float x[kPer];
+    bool counts;
+
+    __device__ __forceinline__ void load(const BalanceArgs& a, uint64_t token, uint32_t lane)
+    {
+        const bool there = token < a.token_count;
+        const float* logits = a.logits + (there ? token : 0u) * a.expert_count;
+        counts = there && token_counts(a, token);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            x[i] = there && lane + 32u * i < a.expert_count ? logits[lane + 32u * i] : 0.0f;
+    }
+};
 // what scores that sum to `total` are multiplied with; scores that are all zero stay zero
 __device__ __forceinline__ float factor_of(float total)
 {
@@ -125,7 +143,7 @@ __device__ __forceinline__ void count_routes(const BalanceArgs& a, uint32_t* off
             atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
             continue;
         }
-        if (!counts(a, token))
+        if (!token_counts(a, token))
             continue;
         uint32_t low = 0, high = experts; // the last expert whose range begins at or before the route
         while (high - low > 1u)
@@ -176,7 +194,7 @@ __device__ __forceinline__ void store_loss(const BalanceArgs& a, const LossParts
 // registers (kPer of each; kPer 0: in shared memory).  The blocks' sums go to scratch, or, where one block has all tokens,
 // straight into the results.
 template<int kFunction, int kPer>
-__global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const BalanceArgs a)
+__global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(const BalanceArgs a)
 {
     extern __shared__ __align__(16) unsigned char shared_raw[];
     const uint32_t experts = a.expert_count;
@@ -200,20 +218,22 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const 
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             sum[i] = 0.0f;
+        LaneRow<kPer> next;
+        next.load(a, first, lane);
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            if (!counts(a, token))
+            const LaneRow<kPer> row = next;
+            next.load(a, token + stride, lane);
+            if (!row.counts)
                 continue;
             ++counted;
-            const float* logits = a.logits + token * experts;
             float x[kPer];
             float peak = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
             {
-                const uint32_t e = lane + 32u * i;
-                x[i] = e < experts ? logits[e] : 0.0f;
-                if (e < experts)
+                x[i] = row.x[i];
+                if (lane + 32u * i < experts)
                     peak = fmaxf(peak, x[i]);
             }
             if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
@@ -245,7 +265,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_partial_kernel(const 
             sum_row[e] = 0.0f;
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            if (!counts(a, token))
+            if (!token_counts(a, token))
                 continue;
             ++counted;
             const float* logits = a.logits + token * experts;
@@ -357,7 +377,7 @@ __global__ void __launch_bounds__(1024) balance_reduce_kernel(const BalanceArgs 
 // ---- backward -----------------------------------------------------------------------------
 
 template<int kFunction, int kPer>
-__global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const BalanceArgs a, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient)
+__global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(const BalanceArgs a, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient)
 {
     extern __shared__ __align__(16) unsigned char shared_raw[];
     const uint32_t experts = a.expert_count;
@@ -372,7 +392,10 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
     unsigned long long mine = 0;
     for (uint32_t e = threadIdx.x; e < experts; e += blockDim.x)
         mine += expert_tokens[e];
-    if (mine != 0ull)
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1)
+        mine += __shfl_xor_sync(kFullMask, mine, offset);
+    if (lane == 0)
         atomicAdd(&routes_shared, mine);
     __syncthreads();
     const double counted = static_cast<double>(max(expert_tokens[experts], 1u));
@@ -387,11 +410,15 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             share[i] = lane + 32u * i < experts ? shares[lane + 32u * i] : 0.0f;
+        LaneRow<kPer> next;
+        next.load(a, first, lane);
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
+            const LaneRow<kPer> row = next;
+            next.load(a, token + stride, lane);
             float* target = gradient + token * experts;
-            float x[kPer], slope[kPer];
-            if (!counts(a, token))
+            float slope[kPer];
+            if (!row.counts)
             {
 #pragma unroll
                 for (int i = 0; i < kPer; ++i)
@@ -399,16 +426,11 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
                         target[lane + 32u * i] = 0.0f;
                 continue;
             }
-            const float* logits = a.logits + token * experts;
             float peak = -INFINITY;
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
-            {
-                const uint32_t e = lane + 32u * i;
-                x[i] = e < experts ? logits[e] : 0.0f;
-                if (e < experts)
-                    peak = fmaxf(peak, x[i]);
-            }
+                if (lane + 32u * i < experts)
+                    peak = fmaxf(peak, row.x[i]);
             if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
                 peak = warp_max(peak);
             float total = 0.0f, mean = 0.0f;
@@ -416,7 +438,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
             for (int i = 0; i < kPer; ++i)
             {
                 float score;
-                score_of<kFunction, true>(x[i], peak, score, slope[i]);
+                score_of<kFunction, true>(row.x[i], peak, score, slope[i]);
                 if (lane + 32u * i >= experts)
                     score = 0.0f;
                 total += score;
@@ -441,7 +463,7 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
             float* target = gradient + token * experts;
-            if (!counts(a, token))
+            if (!token_counts(a, token))
             {
                 for (uint32_t e = lane; e < experts; e += 32u)
                     target[e] = 0.0f;
@@ -477,22 +499,18 @@ __global__ void __launch_bounds__(kBalanceThreads) balance_backward_kernel(const
 
 // ---- launches -----------------------------------------------------------------------------
 
-uint32_t warps_for(uint32_t experts)
+uint32_t blocks_for(uint32_t token_count, uint32_t warps, uint32_t most)
 {
-    return experts <= kRegisterExperts ? kBalanceWarps : kWideWarps;
-}
-uint32_t blocks_for(uint32_t token_count, uint32_t experts, uint32_t most)
-{
-    const uint32_t wanted = (token_count + warps_for(experts) - 1u) / warps_for(experts);
+    const uint32_t wanted = (token_count + warps - 1u) / warps;
     return wanted < most ? wanted : most;
 }
 
 template<int kFunction, int kPer>
 cudaError_t launch_forward(const BalanceArgs& a, cudaStream_t stream)
 {
-    const uint32_t warps = warps_for(a.expert_count);
+    constexpr uint32_t warps = kThreadsFor<kPer> / 32;
     // one block alone (and no second launch) for up to four tokens a warp
-    const uint32_t blocks = a.token_count <= 4u * warps ? 1u : blocks_for(a.token_count, a.expert_count, MOE_BALANCE_MAX_BLOCKS);
+    const uint32_t blocks = a.token_count <= 4u * warps ? 1u : blocks_for(a.token_count, warps, MOE_BALANCE_MAX_BLOCKS);
     const size_t shared_bytes = sizeof(uint32_t) * (2u * a.expert_count + 1u) + sizeof(float) * (kPer > 0 ? 1u : 2u) * warps * a.expert_count;
     static SharedOptIn opt_in;
     if (shared_bytes > 48u * 1024u)
@@ -512,8 +530,8 @@ struct BackwardArgs
 template<int kFunction, int kPer>
 cudaError_t launch_backward(const BalanceArgs& a, const BackwardArgs& b, cudaStream_t stream)
 {
-    const uint32_t warps = warps_for(a.expert_count);
-    return launch_following(balance_backward_kernel<kFunction, kPer>, blocks_for(a.token_count, a.expert_count, 148u * 4u), warps * 32u, sizeof(float) * a.expert_count, stream, a,
+    constexpr uint32_t warps = kThreadsFor<kPer> / 32;
+    return launch_following(balance_backward_kernel<kFunction, kPer>, blocks_for(a.token_count, warps, 148u * 4u), warps * 32u, sizeof(float) * a.expert_count, stream, a,
                             b.expert_tokens, b.loss_gradient, b.gradient);
 }
 

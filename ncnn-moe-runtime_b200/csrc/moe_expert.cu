@@ -70,9 +70,11 @@ struct Eight
 
 // ---- quantisation -------------------------------------------------------------------
 //
-// scale = max |x| / 448 over a block of 128 columns, value = e4m3(x / scale): memory bound (the rows in, a byte a value
-// out).  Sixteen lanes own a block, eight values each, so that a bf16 row is read in 16-byte vectors; a warp takes 1024
-// columns of a row and has all their loads in flight before the first maximum.
+// scale = max |x| / 448 over a block of 128 columns, value = e4m3(x / scale).  Sixteen lanes own a block, eight values each, so
+// that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row and has all their loads in flight before the
+// first maximum.  Bound by instructions before memory (three quarters of the issue slots), so what belongs to a block is done
+// once for the four blocks of a half warp: their maxima are reduced side by side until a lane has one of them, and it divides
+// and inverts that one.
 
 constexpr int kQuantizeThreads = 256;
 constexpr int kQuantizeSteps = 4;                               // blocks of 128 a half warp takes from one item
@@ -84,9 +86,52 @@ __device__ __forceinline__ uint32_t to_e4m3_pair(float low, float high)
     return __nv_cvt_float2_to_fp8x2(make_float2(low, high), __NV_SATFINITE, __NV_E4M3);
 }
 
+__device__ __forceinline__ float approximate_reciprocal(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// a / b with r = 1 / b rounded to nearest, corrected once with the remainder: the exact quotient times 1 + e, |e| < 2^-45,
+// rounded (the reciprocal and the first product are off by 2^-24 each; the correction multiplies that error with 2^-24, and a
+// remainder of up to 25 bits is rounded itself).
+__device__ __forceinline__ float divide_once(float a, float b, float r)
+{
+    const float q = __fmul_rn(a, r);
+    return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
+}
+
+// gate / (1 + exp(-gate)) * up; the quotient within a unit in the last place
 __device__ __forceinline__ float silu_gate(float gate, float up)
 {
-    return __fmul_rn(__fdiv_rn(gate, 1.0f + expf(-gate)), up);
+    const float below = 1.0f + expf(-gate);
+    // (from 2^126 on the reciprocal leaves the normal numbers; an infinity has no remainder)
+    const float quotient = below < 0x1p60f && gate < INFINITY ? divide_once(gate, below, approximate_reciprocal(below)) : __fdiv_rn(gate, below);
+    return __fmul_rn(quotient, up);
+}
+
+// Whether one correction decides e4m3's rounding as the correctly rounded quotient does.  They differ only where the quotient
+// is within 2^-45 of the middle between two fp32 numbers one of which is a tie of e4m3, a number of five bits: X / S = (m 2^20 +- 1)
+// 2^k (1 + e) with mantissas X, S of 24 bits and m of five.  Then X 2^j - S (m 2^20 +- 1) is a whole number of at most 16, so S is
+// within 16 of a multiple of 2^20.
+__device__ __forceinline__ bool correction_decides(float scale)
+{
+    return ((__float_as_uint(scale) + 32u) & 0xFFFFFu) > 64u;
+}
+
+// The maximum of each of a half warp's four values over its lanes: the lane `sub` gets that of value sub / 4.
+__device__ __forceinline__ float reduce_blocks(const float (&top)[4], uint32_t sub)
+{
+    const bool upper = (sub & 8u) != 0u;
+    float a = upper ? top[2] : top[0], b = upper ? top[3] : top[1];
+    a = fmaxf(a, __shfl_xor_sync(kFullMask, upper ? top[0] : top[2], 8));
+    b = fmaxf(b, __shfl_xor_sync(kFullMask, upper ? top[1] : top[3], 8));
+    const bool odd = (sub & 4u) != 0u;
+    float c = odd ? b : a;
+    c = fmaxf(c, __shfl_xor_sync(kFullMask, odd ? a : b, 4));
+    c = fmaxf(c, __shfl_xor_sync(kFullMask, c, 2));
+    return fmaxf(c, __shfl_xor_sync(kFullMask, c, 1));
 }
 
 template<typename T, bool kGate, bool kVector>
@@ -137,54 +182,60 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
                     up[s].load_scalars(source + a.columns + column, count);
             }
         }
+        float x[kQuantizeSteps][8];
+        float top[kQuantizeSteps];
 #pragma unroll
         for (int s = 0; s < kQuantizeSteps; ++s)
         {
-            const uint32_t block_begin = first + 256u * s + 128u * half;
-            const uint32_t column = block_begin + 8u * sub;
-            float x[8];
-            gate[s].unpack(x);
+            gate[s].unpack(x[s]);
             if constexpr (kGate)
             {
                 float y[8];
                 up[s].unpack(y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    x[i] = silu_gate(x[i], y[i]);
+                    x[s][i] = silu_gate(x[s][i], y[i]);
             }
-            float top = 0.0f;
+            top[s] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                top = fmaxf(top, fabsf(x[i]));
-#pragma unroll
-            for (int offset = 8; offset > 0; offset >>= 1)
-                top = fmaxf(top, __shfl_xor_sync(kFullMask, top, offset));
-            const float scale = __fdiv_rn(top, kE4m3Max);
-            // A block of zeros, or one whose scale underflows, converts as it is: zeros, and NaN where there is one.
-            // Quotients are the division's: ties in e4m3 are common among bf16 rows and hang on the last bit.  divide_by
-            // needs a fifth of its instructions; a dividend below its range gives a quotient far below e4m3's smallest.
-            if (scale >= 0x1p-24f && scale < 0x1p25f)
-            {
-                const float reciprocal = __frcp_rn(scale);
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[i] = divide_by(x[i], scale, reciprocal);
-            }
-            else if (scale > 0.0f)
-            {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    x[i] = __fdiv_rn(x[i], scale);
-            }
-            if (block_begin >= a.columns)
-                continue;
-            if (sub == 0u)
+                top[s] = fmaxf(top[s], fabsf(x[s][i]));
+        }
+        static_assert(kQuantizeSteps == 4, "a lane divides for one block of four");
+        const float scale = __fdiv_rn(reduce_blocks(top, sub), kE4m3Max);
+        {
+            const uint32_t block_begin = first + 256u * (sub >> 2) + 128u * half; // the block that this lane divides for
+            if ((sub & 3u) == 0u && block_begin < a.columns)
                 a.scales[static_cast<size_t>(block_begin / MOE_EXPERT_BLOCK) * a.rows + row] = scale;
+        }
+        // A block of zeros, or one whose scale underflows, is divided by one: zeros, and NaN where there is one.
+        const float divisor = scale == 0.0f ? 1.0f : scale;
+        const float reciprocal = __frcp_rn(divisor);
+        // Quotients round as the division's: ties in e4m3 are common among bf16 rows and hang on the last bit.  (In this range the
+        // remainders are exact as above; a dividend too small for that gives a quotient far below e4m3's smallest.)
+        const bool short_way = __all_sync(kFullMask, scale == 0.0f || (scale >= 0x1p-24f && scale < 0x1p25f && correction_decides(scale)));
+#pragma unroll
+        for (int s = 0; s < kQuantizeSteps; ++s)
+        {
+            const uint32_t column = first + 256u * s + 128u * half + 8u * sub;
+            const float by = __shfl_sync(kFullMask, divisor, 16u * half + 4u * s), inverse = __shfl_sync(kFullMask, reciprocal, 16u * half + 4u * s);
+            if (short_way)
+            {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[s][i] = divide_once(x[s][i], by, inverse);
+            }
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x[s][i] = __fdiv_rn(x[s][i], by);
+            }
             if (column >= a.columns)
                 continue;
             uint32_t packed[2];
-            packed[0] = to_e4m3_pair(x[0], x[1]) | (to_e4m3_pair(x[2], x[3]) << 16);
-            packed[1] = to_e4m3_pair(x[4], x[5]) | (to_e4m3_pair(x[6], x[7]) << 16);
+            packed[0] = to_e4m3_pair(x[s][0], x[s][1]) | (to_e4m3_pair(x[s][2], x[s][3]) << 16);
+            packed[1] = to_e4m3_pair(x[s][4], x[s][5]) | (to_e4m3_pair(x[s][6], x[s][7]) << 16);
             uint8_t* target = a.values + static_cast<size_t>(row) * a.columns + column;
             if constexpr (kVector)
                 *reinterpret_cast<uint2*>(target) = make_uint2(packed[0], packed[1]);
