@@ -17,10 +17,17 @@ namespace moe {
 namespace {
 
 constexpr uint32_t kRegisterExperts = 1024; // up to here a lane holds a row's scores in registers
-// Threads of a block by the scores a lane holds: two or four blocks to an SM; rows in shared memory (kPer 0) need 32 bytes a
-// warp and expert.
+// Threads of a block by the scores a lane holds; rows in shared memory (kPer 0) need 32 bytes a warp and expert.
 template<int kPer>
-constexpr int kThreadsFor = kPer == 0 ? 128 : kPer >= 32 ? 256 : 512;
+constexpr int kThreadsFor = kPer == 0 ? 128 : 512;
+// Whether the next token's logits are requested while one is worked on: 65536 x 256, gradient, 30 against 38 us.  32 scores a lane
+// leave no registers for it (32768 x 1024, loss, 69 against 54 us).
+template<int kPer>
+constexpr bool kAhead = kPer <= 16;
+// One wave of blocks: with twice as many, the second half waits for registers (65536 x 256, loss, 28 against 31 us; 32768 x 512
+// 34 against 43).
+template<int kPer>
+constexpr uint32_t kMostBlocks = kPer == 0 || kPer >= 16 ? 148u : MOE_BALANCE_MAX_BLOCKS;
 
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -134,17 +141,18 @@ __device__ __forceinline__ void count_routes(const BalanceArgs& a, uint32_t* off
             atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
         return;
     }
+    // a warp has 32 routes in a row, which mostly belong to one expert: one addition for all of them
+    const uint32_t lane = threadIdx.x & 31u;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x;
-    for (uint64_t route = offsets[0] + static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; route < offsets[experts]; route += stride)
+    const uint64_t end = offsets[experts];
+    for (uint64_t base = offsets[0] + static_cast<uint64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31u); base < end; base += stride)
     {
-        const uint32_t token = a.route_token[route];
-        if (token >= a.token_count)
-        {
+        const uint64_t route = base + lane;
+        const uint32_t token = route < end ? a.route_token[route] : 0u;
+        bool valid = route < end && token < a.token_count;
+        if (route < end && !valid)
             atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
-            continue;
-        }
-        if (!token_counts(a, token))
-            continue;
+        valid = valid && token_counts(a, token);
         uint32_t low = 0, high = experts; // the last expert whose range begins at or before the route
         while (high - low > 1u)
         {
@@ -154,7 +162,17 @@ __device__ __forceinline__ void count_routes(const BalanceArgs& a, uint32_t* off
             else
                 high = middle;
         }
-        atomicAdd(&routed[low], 1u);
+        const uint32_t expert = __shfl_sync(kFullMask, low, 0);
+        const unsigned votes = __ballot_sync(kFullMask, valid);
+        if (__all_sync(kFullMask, low == expert || !valid))
+        {
+            if (lane == 0)
+                atomicAdd(&routed[expert], static_cast<uint32_t>(__popc(votes)));
+        }
+        else if (valid)
+        {
+            atomicAdd(&routed[low], 1u);
+        }
     }
 }
 
@@ -207,10 +225,13 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(cons
     if (threadIdx.x == 0)
         counted_shared = 0u;
     wait_for_previous_kernel();
+    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * warps + warp, stride = static_cast<uint64_t>(gridDim.x) * warps;
+    LaneRow<kPer == 0 ? 1 : kPer> next;
+    if constexpr (kPer > 0 && kAhead<kPer>)
+        next.load(a, first, lane);
     count_routes(a, offsets, routed);
 
     uint32_t counted = 0;
-    const uint64_t first = static_cast<uint64_t>(blockIdx.x) * warps + warp, stride = static_cast<uint64_t>(gridDim.x) * warps;
     float* const sum_row = sums + static_cast<size_t>(warp) * experts;
     if constexpr (kPer > 0)
     {
@@ -218,12 +239,18 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(cons
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             sum[i] = 0.0f;
-        LaneRow<kPer> next;
-        next.load(a, first, lane);
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            const LaneRow<kPer> row = next;
-            next.load(a, token + stride, lane);
+            LaneRow<kPer> row;
+            if constexpr (kAhead<kPer>)
+            {
+                row = next;
+                next.load(a, token + stride, lane);
+            }
+            else
+            {
+                row.load(a, token, lane);
+            }
             if (!row.counts)
                 continue;
             ++counted;
@@ -406,16 +433,25 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(con
     const uint64_t first = static_cast<uint64_t>(blockIdx.x) * warps + warp, stride = static_cast<uint64_t>(gridDim.x) * warps;
     if constexpr (kPer > 0)
     {
+        LaneRow<kPer> next;
+        if constexpr (kAhead<kPer>)
+            next.load(a, first, lane);
         float share[kPer];
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
             share[i] = lane + 32u * i < experts ? shares[lane + 32u * i] : 0.0f;
-        LaneRow<kPer> next;
-        next.load(a, first, lane);
         for (uint64_t token = first; token < a.token_count; token += stride)
         {
-            const LaneRow<kPer> row = next;
-            next.load(a, token + stride, lane);
+            LaneRow<kPer> row;
+            if constexpr (kAhead<kPer>)
+            {
+                row = next;
+                next.load(a, token + stride, lane);
+            }
+            else
+            {
+                row.load(a, token, lane);
+            }
             float* target = gradient + token * experts;
             float slope[kPer];
             if (!row.counts)
@@ -510,7 +546,7 @@ cudaError_t launch_forward(const BalanceArgs& a, cudaStream_t stream)
 {
     constexpr uint32_t warps = kThreadsFor<kPer> / 32;
     // one block alone (and no second launch) for up to four tokens a warp
-    const uint32_t blocks = a.token_count <= 4u * warps ? 1u : blocks_for(a.token_count, warps, MOE_BALANCE_MAX_BLOCKS);
+    const uint32_t blocks = a.token_count <= 4u * warps ? 1u : blocks_for(a.token_count, warps, kMostBlocks<kPer>);
     const size_t shared_bytes = sizeof(uint32_t) * (2u * a.expert_count + 1u) + sizeof(float) * (kPer > 0 ? 1u : 2u) * warps * a.expert_count;
     static SharedOptIn opt_in;
     if (shared_bytes > 48u * 1024u)
@@ -531,7 +567,7 @@ template<int kFunction, int kPer>
 cudaError_t launch_backward(const BalanceArgs& a, const BackwardArgs& b, cudaStream_t stream)
 {
     constexpr uint32_t warps = kThreadsFor<kPer> / 32;
-    return launch_following(balance_backward_kernel<kFunction, kPer>, blocks_for(a.token_count, warps, 148u * 4u), warps * 32u, sizeof(float) * a.expert_count, stream, a,
+    return launch_following(balance_backward_kernel<kFunction, kPer>, blocks_for(a.token_count, warps, kMostBlocks<kPer>), warps * 32u, sizeof(float) * a.expert_count, stream, a,
                             b.expert_tokens, b.loss_gradient, b.gradient);
 }
 

@@ -76,7 +76,7 @@ struct Eight
 // once for the four blocks of a half warp: their maxima are reduced side by side until a lane has one of them, and it divides
 // and inverts that one.
 
-constexpr int kQuantizeThreads = 256;
+constexpr int kQuantizeThreads = 128;
 constexpr int kQuantizeSteps = 4;                               // blocks of 128 a half warp takes from one item
 constexpr uint32_t kQuantizeItem = 256u * kQuantizeSteps;       // columns of an item
 constexpr float kE4m3Max = 448.0f;
@@ -294,7 +294,7 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
     const bool vector = a.columns % 8u == 0u && bases % 16u == 0u && a.row_stride * sizeof(T) % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 8u == 0u;
     const uint64_t items = static_cast<uint64_t>(a.rows) * ((a.columns + kQuantizeItem - 1u) / kQuantizeItem);
     const uint64_t blocks = (items + kQuantizeThreads / 32 - 1) / (kQuantizeThreads / 32);
-    const uint32_t grid = static_cast<uint32_t>(blocks < 148u * 8u ? blocks : 148u * 8u);
+    const uint32_t grid = static_cast<uint32_t>(blocks < 148u * 16u ? blocks : 148u * 16u);
     auto kernel = gate ? (vector ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, true, false>)
                        : (vector ? quantize_rows_kernel<T, false, true> : quantize_rows_kernel<T, false, false>);
     return launch_following(kernel, grid, kQuantizeThreads, 0, stream, a);

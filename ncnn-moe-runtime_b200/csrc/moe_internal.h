@@ -17,8 +17,8 @@
 #define MOE_SPECULATIVE_SHORT_LIST 1024u
 // entries of the router's [expert][block] count table (expert_count * blocks of the select kernel never exceeds it)
 #define MOE_ROUTER_BLOCK_TABLE_ENTRIES 262144u
-// blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): four per SM
-#define MOE_BALANCE_MAX_BLOCKS 592u
+// blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): two per SM
+#define MOE_BALANCE_MAX_BLOCKS 296u
 
 namespace moe {
 
