@@ -6,8 +6,8 @@
 // one fused multiply-add per element of the tile and block.  Two kernels:
 //   few rows an expert   a tile is 128 outputs (the 128 lanes of an accumulator) by 16, 32 or 64 rows (its columns): the rows of
 //                        a decode step do not fill a tile of 128 with padding.  Bound by the weights from HBM.
-//   many rows            a tile is 128 rows by 256 outputs, or 256 by 256 on a pair of SMs: a thread sums for one row, so that a
-//                        block's factor is one register.  Bound by the tensor cores, by L2 or by the weights.
+//   many rows            a tile is 128 rows by 256 outputs: a thread sums for one row, so that a block's factor is one register.
+//                        Bound by the sums or by the weights.
 // Roles of a CTA, which stays for all its tiles: a thread that requests tiles of both operands from the copy engine, threads
 // that issue the products, warps that scale, sum and store.  They pass a ring of operand stages and a few accumulators to each
 // other through mbarriers, so that copies, products and sums of different blocks, and of different tiles, overlap.
@@ -133,10 +133,10 @@ struct ProductRings
 };
 
 // Issues the products of `count` blocks in a row, the first of them block `block` of its tile.  One thread.
-template<bool kPair, uint32_t kStages, uint32_t kStageBytes, uint32_t kAccumulators, uint32_t kWide>
+template<uint32_t kStages, uint32_t kStageBytes, uint32_t kAccumulators, uint32_t kWide>
 __device__ __forceinline__ void issue_products(const ProductRings& rings, uint32_t memory_base, uint32_t count, uint32_t block, uint32_t columns, volatile uint32_t* stalled)
 {
-    constexpr uint32_t kDescriptor = product_descriptor(kPair ? 2u * kLanes : kLanes, kWide);
+    constexpr uint32_t kDescriptor = product_descriptor(kLanes, kWide);
     const uint32_t blocks = (columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
     const uint32_t last_steps = (columns - (blocks - 1u) * MOE_EXPERT_BLOCK + 31u) / 32u;
     Cursor cursor, sum;
@@ -154,9 +154,9 @@ __device__ __forceinline__ void issue_products(const ProductRings& rings, uint32
 #pragma unroll
         for (uint32_t step = 0; step < 4u; ++step)
             if (step < steps)
-                issue_product<kPair>(memory_base + sum.slot * kWide, tall + 2u * step, wide + 2u * step, kDescriptor, step != 0u);
-        commit_products<kPair>(rings.empty + 8u * cursor.slot);
-        commit_products<kPair>(rings.sum_full + 8u * sum.slot);
+                issue_product(memory_base + sum.slot * kWide, tall + 2u * step, wide + 2u * step, kDescriptor, step != 0u);
+        commit_products(rings.empty + 8u * cursor.slot);
+        commit_products(rings.sum_full + 8u * sum.slot);
         cursor.advance(kStages);
         sum.advance(kAccumulators);
     }
@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
         barrier_init_fence();
     }
     if (warp == 3u)
-        allocate_memory<false>(shared_address(&memory_base_shared), S::kMemoryColumns);
-    memory_sync<false>();
+        allocate_memory(shared_address(&memory_base_shared), S::kMemoryColumns);
+    memory_sync();
     const uint32_t memory_base = memory_base_shared;
 
     wait_for_previous_kernel();
@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
                     const uint32_t stage = rings.stages + cursor.slot * S::kStageBytes;
                     const uint32_t barrier = rings.full + 8u * cursor.slot;
                     barrier_expect_bytes(barrier, S::kStageBytes);
-                    copy_tile<false>(stage, &weight_map, block * kBlockBytes, weight_row, barrier);
-                    copy_tile<false>(stage + kTallTile, &row_map, block * kBlockBytes, tile.first_row, barrier);
+                    copy_tile(stage, &weight_map, block * kBlockBytes, weight_row, barrier);
+                    copy_tile(stage + kTallTile, &row_map, block * kBlockBytes, tile.first_row, barrier);
                     cursor.advance(S::kStages);
                     ++issued;
                 }
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
     else if (warp == 1u)
     {
         if (elect_one())
-            issue_products<false, S::kStages, S::kStageBytes, S::kAccumulators, kTokens>(
+            issue_products<S::kStages, S::kStageBytes, S::kAccumulators, kTokens>(
                 rings, memory_base, first < tiles ? ((tiles - first - 1u) / stride + 1u) * (end - begin) : 0u, begin, a.columns, &stalled);
     }
     else if (warp == 2u)
@@ -474,9 +474,9 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
             }
         }
     }
-    memory_sync<false>();
+    memory_sync();
     if (warp == 3u)
-        free_memory<false>(memory_base, S::kMemoryColumns);
+        free_memory(memory_base, S::kMemoryColumns);
     if (threadIdx.x == 0 && stalled != 0u)
         atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
     if (split > 1u)
@@ -523,16 +523,10 @@ __global__ void __launch_bounds__(FewShape<kTokens>::kThreads, 1)
 
 constexpr uint32_t kTileOutputs = 256;
 
-// kPair: two CTAs of a cluster share a tile of 256 rows.  Each has its 128 rows and the weights of half of the outputs in its
-// shared memory; the first one issues products that read both halves and write both tensor memories.
-template<bool kPair>
 struct ManyShape
 {
-    static constexpr uint32_t kCtas = kPair ? 2u : 1u;
-    static constexpr uint32_t kTileRows = kLanes * kCtas;
-    static constexpr uint32_t kWeightBox = kTileOutputs / kCtas; // weight rows that a CTA copies
-    static constexpr uint32_t kStageBytes = kTallTile + kWeightBox * kBlockBytes;
-    static constexpr uint32_t kStages = kPair ? 6u : 4u;
+    static constexpr uint32_t kStageBytes = kTallTile + kTileOutputs * kBlockBytes;
+    static constexpr uint32_t kStages = 4;
     static constexpr uint32_t kAccumulators = 2;
     static constexpr uint32_t kMemoryColumns = kTileOutputs * kAccumulators;
     static constexpr uint32_t kSumWarps = 8;
@@ -563,11 +557,11 @@ __device__ __forceinline__ void store_outputs(__nv_bfloat16* target, const float
     }
     *reinterpret_cast<uint4*>(target) = make_uint4(words[0], words[1], words[2], words[3]);
 }
-template<bool kPair, typename Out>
-__global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
+template<typename Out>
+__global__ void __launch_bounds__(ManyShape::kThreads, 1)
     expert_product_many_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
 {
-    using S = ManyShape<kPair>;
+    using S = ManyShape;
     extern __shared__ unsigned char shared_raw[];
     __shared__ uint32_t memory_base_shared;
     __shared__ volatile uint32_t stalled;
@@ -580,7 +574,6 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
     rings.sum_empty = rings.sum_full + 8u * S::kAccumulators;
     uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + 8u * S::kBarriers);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t cta = kPair ? cta_in_cluster() : 0u; // of the pair
 
     if (threadIdx.x == 0)
     {
@@ -592,27 +585,26 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
         for (uint32_t i = 0; i < S::kAccumulators; ++i)
         {
             barrier_init(rings.sum_full + 8u * i, 1u);
-            barrier_init(rings.sum_empty + 8u * i, S::kSumWarps * S::kCtas);
+            barrier_init(rings.sum_empty + 8u * i, S::kSumWarps);
         }
         stalled = 0u;
         barrier_init_fence();
     }
     __syncwarp();
     if (warp == 3u)
-        allocate_memory<kPair>(shared_address(&memory_base_shared), S::kMemoryColumns);
-    memory_sync<kPair>();
+        allocate_memory(shared_address(&memory_base_shared), S::kMemoryColumns);
+    memory_sync();
     const uint32_t memory_base = memory_base_shared;
 
     wait_for_previous_kernel();
     const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
     const uint32_t output_blocks = (a.outputs + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
     const uint32_t output_tiles = (a.outputs + kTileOutputs - 1u) / kTileOutputs;
-    const bool good = count_tiles<S::kTileRows>(a, first_tile, output_tiles);
+    const bool good = count_tiles<kLanes>(a, first_tile, output_tiles);
     __syncthreads();
     const uint32_t tiles = good ? first_tile[a.expert_count] : 0u;
     if (!good && threadIdx.x == 0)
         atomicOr(a.flags, MOE_EXPERT_FLAG_OFFSETS);
-    const uint32_t first = blockIdx.x / S::kCtas, stride = gridDim.x / S::kCtas;
 
     if (warp < 4u)
     {
@@ -623,39 +615,32 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
             {
                 Cursor cursor;
                 uint32_t issued = 0;
-                for (uint32_t t = first; t < tiles && stalled == 0u; t += stride)
+                for (uint32_t t = blockIdx.x; t < tiles && stalled == 0u; t += gridDim.x)
                 {
-                    const Tile tile = find_tile<S::kTileRows>(a, first_tile, t, output_tiles);
+                    const Tile tile = find_tile<kLanes>(a, first_tile, t, output_tiles);
                     // what lies past an expert's rows or outputs belongs to the next one, or is zero: it is not stored
-                    const uint32_t weight_row = tile.expert * a.outputs + tile.output_tile * kTileOutputs + cta * S::kWeightBox;
-                    const uint32_t row = tile.first_row + cta * kLanes;
+                    const uint32_t weight_row = tile.expert * a.outputs + tile.output_tile * kTileOutputs;
                     for (uint32_t block = 0; block < blocks; ++block)
                     {
                         if (!barrier_wait(rings.empty + 8u * cursor.slot, cursor.parity ^ 1u, &stalled))
                             break;
                         const uint32_t stage = rings.stages + cursor.slot * S::kStageBytes;
-                        uint32_t barrier = rings.full + 8u * cursor.slot;
-                        if (cta == 0u)
-                            barrier_expect_bytes(barrier, S::kStageBytes * S::kCtas);
-                        else
-                            barrier = barrier_of_cta(barrier, 0u);
-                        copy_tile<kPair>(stage, &row_map, block * kBlockBytes, row, barrier);
-                        copy_tile<kPair>(stage + kTallTile, &weight_map, block * kBlockBytes, weight_row, barrier);
+                        const uint32_t barrier = rings.full + 8u * cursor.slot;
+                        barrier_expect_bytes(barrier, S::kStageBytes);
+                        copy_tile(stage, &row_map, block * kBlockBytes, tile.first_row, barrier);
+                        copy_tile(stage + kTallTile, &weight_map, block * kBlockBytes, weight_row, barrier);
                         cursor.advance(S::kStages);
                         ++issued;
                     }
                 }
-                // (The second CTA of a pair has seen its copies used, or a wait run out that is far longer than a copy takes.)
-                if (cta == 0u)
-                    wait_for_copies(rings.full, cursor, S::kStages, issued);
+                wait_for_copies(rings.full, cursor, S::kStages, issued);
             }
         }
         else if (warp == 1u)
         {
-            if (cta == 0u)
-                if (elect_one())
-                    issue_products<kPair, S::kStages, S::kStageBytes, S::kAccumulators, kTileOutputs>(
-                        rings, memory_base, first < tiles ? ((tiles - first - 1u) / stride + 1u) * blocks : 0u, 0u, a.columns, &stalled);
+            if (elect_one())
+                issue_products<S::kStages, S::kStageBytes, S::kAccumulators, kTileOutputs>(
+                    rings, memory_base, blockIdx.x < tiles ? ((tiles - blockIdx.x - 1u) / gridDim.x + 1u) * blocks : 0u, 0u, a.columns, &stalled);
         }
     }
     else
@@ -664,17 +649,18 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
         const uint32_t quarter = warp & 3u;      // lanes of tensor memory that this warp can read
         const uint32_t half = (warp - 4u) / 4u;  // of the tile's outputs
         const uint32_t memory = memory_base + (quarter << 21) + half * S::kColumns;
-        const uint32_t row = cta * kLanes + quarter * 32u + lane; // of a tile
+        const uint32_t row = quarter * 32u + lane; // of a tile
         // The scales are read two blocks ahead, across tiles.  The loads stand outside of any condition (behind the last tile they
         // repeat the last ones): a value that is merged with another one behind a branch is waited for there.
-        uint32_t ahead_tile = first, ahead_block = 0;
+        uint32_t ahead_tile = blockIdx.x, ahead_block = 0;
         const float* ahead_scales = a.scales;
         const float* ahead_weights = a.weight_scales;
         float next_scale[2], next_weight[2];
+        Tile next_tile = {};
         const auto find_scales = [&]() {
             if (ahead_tile < tiles)
             {
-                const Tile tile = find_tile<S::kTileRows>(a, first_tile, ahead_tile, output_tiles);
+                const Tile tile = next_tile = find_tile<kLanes>(a, first_tile, ahead_tile, output_tiles);
                 // (an odd number of blocks: the second half of the last tile has no scales, and is not stored)
                 const uint32_t output_block = min(tile.output_tile * 2u + half, output_blocks - 1u);
                 ahead_weights = a.weight_scales + (static_cast<size_t>(tile.expert) * output_blocks + output_block) * blocks;
@@ -696,17 +682,20 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
             else
             {
                 ahead_block = 0;
-                ahead_tile += stride;
+                ahead_tile += gridDim.x;
                 find_scales();
             }
         };
         find_scales();
-        if (first < tiles)
+        if (blockIdx.x < tiles)
             request();
         Cursor sum;
         bool running = true;
-        for (uint32_t t = first; t < tiles && running; t += stride)
+        for (uint32_t t = blockIdx.x; t < tiles && running; t += gridDim.x)
         {
+            const Tile tile = next_tile;
+            // a warp whose 32 rows are not the expert's only passes the accumulators on
+            const bool idle = quarter * 32u >= tile.rows;
             float sums[S::kColumns];
 #pragma unroll
             for (uint32_t i = 0; i < S::kColumns; ++i)
@@ -723,6 +712,13 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
                     running = barrier_wait_warp(rings.sum_full + 8u * sum.slot, sum.parity, &stalled);
                     if (!running)
                         break;
+                    if (idle)
+                    {
+                        if (lane == 0u)
+                            barrier_arrive(rings.sum_empty + 8u * sum.slot);
+                        sum.advance(S::kAccumulators);
+                        continue;
+                    }
                     memory_fence_after();
                     const uint32_t source = memory + sum.slot * kTileOutputs;
                     const float factor = factors[of_two];
@@ -746,12 +742,7 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
                                 memory_fence_before();
                                 __syncwarp();
                                 if (lane == 0u)
-                                {
-                                    if (cta == 0u)
-                                        barrier_arrive(rings.sum_empty + 8u * sum.slot);
-                                    else
-                                        barrier_arrive_cluster(barrier_of_cta(rings.sum_empty + 8u * sum.slot, 0u));
-                                }
+                                    barrier_arrive(rings.sum_empty + 8u * sum.slot);
                             }
                         }
 #pragma unroll
@@ -765,7 +756,6 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
             }
             if (!running)
                 break;
-            const Tile tile = find_tile<S::kTileRows>(a, first_tile, t, output_tiles);
             const uint32_t output = tile.output_tile * kTileOutputs + half * S::kColumns;
             if (row < tile.rows && output < a.outputs)
             {
@@ -791,9 +781,9 @@ __global__ void __launch_bounds__(ManyShape<kPair>::kThreads, 1)
             }
         }
     }
-    memory_sync<kPair>(); // neither side's shared or tensor memory is used any more
+    memory_sync();
     if (warp == 3u)
-        free_memory<kPair>(memory_base, S::kMemoryColumns);
+        free_memory(memory_base, S::kMemoryColumns);
     if (threadIdx.x == 0 && stalled != 0u)
         atomicOr(a.flags, MOE_EXPERT_FLAG_STALLED);
 }
@@ -874,21 +864,19 @@ cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
         split *= 2u;
     return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, (tiles < most ? tiles * split : most), split, S::kThreads, S::kFixedBytes, stream, split);
 }
-template<bool kPair, typename Out>
+template<typename Out>
 cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
-    using S = ManyShape<kPair>;
+    using S = ManyShape;
     static SharedOptIn opt_in;
-    const uint64_t tiles = most_tiles(a, S::kTileRows, kTileOutputs), most = static_cast<uint64_t>(sm_count) / S::kCtas;
-    return launch_tiles(expert_product_many_kernel<kPair, Out>, opt_in, a, kLanes, S::kWeightBox, (tiles < most ? tiles : most) * S::kCtas, S::kCtas, S::kThreads, S::kFixedBytes, stream);
+    const uint64_t tiles = most_tiles(a, kLanes, kTileOutputs), most = static_cast<uint64_t>(sm_count);
+    return launch_tiles(expert_product_many_kernel<Out>, opt_in, a, kLanes, kTileOutputs, tiles < most ? tiles : most, 1u, S::kThreads, S::kFixedBytes, stream);
 }
 
 // Experts are taken to have equal numbers of rows.  Up to 32 a tile of as many rows wastes least (64 experts of 32 rows x
 // 4096 x 4096: 32-row tiles 172 us, 64-row tiles 204, 128 x 256 tiles 187).  Above that the tiles' rates decide: a block of 64
 // rows by 128 outputs takes three fifths of the time of one of 128 by 256, so the smaller ones win while they are one wave (one
-// expert of 256 rows: 15.5 against 21.8 us) and lose from two on (512 rows: 27.0 against 22.2).  Pairs of SMs read half of
-// the weights each: that pays where many full tiles are bound by L2 (64 experts of 256 rows 367 against 420 us) and costs where
-// tiles of 256 rows are partly empty (128 rows each 351 against 211) or few (one expert of 1024 rows 24.2 against 23.0).
+// expert of 256 rows: 15.5 against 21.8 us) and lose from two on (512 rows: 27.0 against 22.2).
 template<typename Out>
 cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
@@ -902,12 +890,9 @@ cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stre
         const uint64_t tiles = active * ((rows + tile_rows - 1u) / tile_rows) * ((a.outputs + tile_outputs - 1u) / tile_outputs);
         return (tiles + sm_count - 1u) / sm_count;
     };
-    const uint64_t many = waves(kLanes, kTileOutputs);
-    if (waves(64u, kLanes) * 3u <= many * 5u)
+    if (waves(64u, kLanes) * 3u <= waves(kLanes, kTileOutputs) * 5u)
         return launch_few<64, Out>(a, sm_count, stream);
-    if (rows >= 224u && many >= 8u)
-        return launch_many<true, Out>(a, sm_count, stream);
-    return launch_many<false, Out>(a, sm_count, stream);
+    return launch_many<Out>(a, sm_count, stream);
 }
 
 } // namespace

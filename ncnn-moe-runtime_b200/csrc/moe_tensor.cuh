@@ -25,19 +25,6 @@ __device__ __forceinline__ void barrier_arrive(uint32_t barrier)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
-// the same barrier of another CTA of the cluster
-__device__ __forceinline__ uint32_t barrier_of_cta(uint32_t barrier, uint32_t cta)
-{
-    uint32_t address;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(address) : "r"(barrier), "r"(cta));
-    return address;
-}
-// Publishes nothing: what the arrival orders is the read of tensor memory before it.  (A release for the cluster waits for the
-// thread's earlier writes: about 1 us a block.)
-__device__ __forceinline__ void barrier_arrive_cluster(uint32_t barrier_in_cluster)
-{
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(barrier_in_cluster) : "memory");
-}
 __device__ __forceinline__ uint32_t cta_in_cluster()
 {
     uint32_t rank;
@@ -100,18 +87,11 @@ __device__ __forceinline__ bool barrier_wait_warp(uint32_t barrier, uint32_t par
     return false;
 }
 
-// kPair: the bytes are counted at a barrier of either CTA of the pair.
-template<bool kPair>
 __device__ __forceinline__ void copy_tile(uint32_t destination, const CUtensorMap* map, uint32_t column, uint32_t row, uint32_t barrier)
 {
-    if constexpr (kPair)
-        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(destination), "l"(map),
-                     "r"(column), "r"(row), "r"(barrier)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(destination), "l"(map), "r"(column),
-                     "r"(row), "r"(barrier)
-                     : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(destination), "l"(map), "r"(column), "r"(row),
+                 "r"(barrier)
+                 : "memory");
 }
 
 // four bytes, or zeros
@@ -126,41 +106,26 @@ __device__ __forceinline__ uint64_t tile_descriptor(uint32_t address)
 {
     return static_cast<uint64_t>((address & 0x3FFFFu) >> 4) | (1ull << 16) | (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// e4m3 by e4m3 into fp32, both operands with adjacent columns: `tall` lanes (of both CTAs of a pair) by `wide` columns
+// e4m3 by e4m3 into fp32, both operands with adjacent columns: `tall` lanes by `wide` columns
 __device__ __forceinline__ constexpr uint32_t product_descriptor(uint32_t tall, uint32_t wide)
 {
     return (1u << 4) | ((wide >> 3) << 17) | ((tall >> 4) << 24);
 }
-template<bool kPair>
 __device__ __forceinline__ void issue_product(uint32_t accumulator, uint64_t tall, uint64_t wide, uint32_t descriptor, bool accumulate)
 {
-    if constexpr (kPair)
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "setp.ne.u32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-            "}\n" ::"r"(accumulator),
-            "l"(tall), "l"(wide), "r"(descriptor), "r"(accumulate ? 1u : 0u)
-            : "memory");
-    else
-        asm volatile(
-            "{\n"
-            ".reg .pred p;\n"
-            "setp.ne.u32 p, %4, 0;\n"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-            "}\n" ::"r"(accumulator),
-            "l"(tall), "l"(wide), "r"(descriptor), "r"(accumulate ? 1u : 0u)
-            : "memory");
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.u32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(accumulator),
+        "l"(tall), "l"(wide), "r"(descriptor), "r"(accumulate ? 1u : 0u)
+        : "memory");
 }
-// arrives at the barrier (of both CTAs of a pair) once the products issued so far are done
-template<bool kPair>
+// arrives at the barrier once the products issued so far are done
 __device__ __forceinline__ void commit_products(uint32_t barrier)
 {
-    if constexpr (kPair)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(barrier), "h"(static_cast<uint16_t>(3)) : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
 }
 
 template<int kCount>
@@ -231,28 +196,15 @@ struct Cursor
     }
 };
 
-// Columns of tensor memory for the CTA (kPair: for both CTAs of a pair, called by a warp of each); whole warps.
-template<bool kPair>
+// Columns of tensor memory for the CTA; whole warps.
 __device__ __forceinline__ void allocate_memory(uint32_t base_address, uint32_t columns)
 {
-    if constexpr (kPair)
-    {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base_address), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
-    else
-    {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base_address), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base_address), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-template<bool kPair>
 __device__ __forceinline__ void free_memory(uint32_t base, uint32_t columns)
 {
-    if constexpr (kPair)
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
-    else
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void memory_fence_before()
 {
@@ -262,16 +214,12 @@ __device__ __forceinline__ void memory_fence_after()
 {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// All threads of the CTA (of both CTAs of a pair), with what they did to tensor memory.
-template<bool kPair>
+// All threads of the CTA, with what they did to tensor memory.
 __device__ __forceinline__ void memory_sync()
 {
     __syncwarp();
     memory_fence_before();
-    if constexpr (kPair)
-        cluster_sync();
-    else
-        __syncthreads();
+    __syncthreads();
     memory_fence_after();
 }
 
