@@ -414,8 +414,9 @@ enum moe_activation
  *              MOE_EXPERT_FLAG_TOKEN_RANGE.
  * values       device, [rows x columns] e4m3, dense
  * scales       device, [ceil(columns / 128) x rows]: block-major
- * Asynchronous on `stream`.  Calls that route their source rows twice or more on average may quantise each row once
- * and grow the handle's scratch for that (at most 48 MiB); make the largest one before a stream capture. */
+ * columns and rows < 2^31.  Asynchronous on `stream`.  Calls that route their source rows twice or more on average may
+ * quantise each row once and grow the handle's scratch for that (48 MiB at most a call); scratch grows outside of stream
+ * captures, so make the largest call before one.  Graphs captured earlier stay valid. */
 int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,
                       int activation, const uint32_t* route_token, uint32_t route_count, uint8_t* values, float* scales);
 
@@ -450,7 +451,8 @@ int moe_expert_product(moe_sampler* sampler, void* stream, const uint8_t* values
  * base         device, [token_count x columns] of dtype, or NULL; may be `out`
  * out          device, [token_count x columns] of dtype, not overlapping route_rows; a token without routes gets its base, or zeros
  * top_k <= MOE_EXPERT_MAX_EXPERTS.  Asynchronous on `stream`.  Calls with more routes than any before on this handle grow its scratch
- * (token_count * top_k words); make the largest one before a stream capture. */
+ * (token_count * top_k words) outside of stream captures; make the largest one before a capture.  Graphs captured earlier
+ * stay valid. */
 int moe_combine_routes(moe_sampler* sampler, void* stream, const void* route_rows, int dtype, size_t row_stride, uint32_t columns,
                        const uint32_t* route_token, const uint32_t* route_rank, const float* route_weight, uint32_t route_count, uint32_t token_count,
                        uint32_t top_k, const void* base, void* out);

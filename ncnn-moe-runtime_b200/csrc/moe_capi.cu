@@ -83,6 +83,7 @@ struct moe_sampler
     uint32_t* balance_counts = nullptr;
     size_t balance_sums_capacity = 0;
     size_t balance_counts_capacity = 0;
+    std::vector<void*> kept_scratch;   // what grow_kept replaced
     // router host staging
     float* router_logits_dev = nullptr;
     size_t router_logits_capacity = 0;
@@ -140,6 +141,32 @@ cudaError_t grow(T*& pointer, size_t& capacity, size_t wanted)
     cudaError_t status = cudaMalloc(reinterpret_cast<void**>(&pointer), entries * sizeof(T));
     if (status == cudaSuccess)
         capacity = entries;
+    return status;
+}
+
+// Scratch of calls that may be captured: what a captured graph was given stays allocated until the handle goes, so a later,
+// larger call does not take it away.  At least doubled each time, so all of it together stays below twice the largest.
+template<typename T>
+cudaError_t grow_kept(std::vector<void*>& kept, T*& pointer, size_t& capacity, size_t wanted)
+{
+    const size_t entries = wanted > 2u * capacity ? wanted : 2u * capacity;
+    try
+    {
+        kept.reserve(kept.size() + 1u); // no exception may leave a C entry point
+    }
+    catch (const std::bad_alloc&)
+    {
+        return cudaErrorMemoryAllocation;
+    }
+    T* larger = nullptr;
+    cudaError_t status = cudaMalloc(reinterpret_cast<void**>(&larger), entries * sizeof(T));
+    if (status == cudaSuccess)
+    {
+        if (pointer != nullptr)
+            kept.push_back(pointer);
+        pointer = larger;
+        capacity = entries;
+    }
     return status;
 }
 
@@ -366,6 +393,8 @@ void moe_sampler_destroy(moe_sampler* sampler)
     for (void* pointer : pointers)
         if (pointer != nullptr)
             cudaFree(pointer);
+    for (void* pointer : sampler->kept_scratch)
+        cudaFree(pointer);
     if (sampler->sampled_host != nullptr)
         cudaFreeHost(sampler->sampled_host);
     if (sampler->stream != nullptr)
@@ -1071,11 +1100,7 @@ int moe_quantize_rows(moe_sampler* sampler, void* stream_handle, const void* sou
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     const size_t once = quantize_once_bytes(args);
     if (once > sampler->quantize_once_capacity)
-    {
-        // earlier calls on this stream may still use the scratch that is replaced here
-        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
-        MOE_CUDA_CHECK(sampler, grow(sampler->quantize_once, sampler->quantize_once_capacity, once));
-    }
+        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->quantize_once, sampler->quantize_once_capacity, once));
     MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, once > 0 ? sampler->quantize_once : nullptr, stream));
     return MOE_STATUS_OK;
 }
@@ -1112,10 +1137,8 @@ int moe_combine_routes(moe_sampler* sampler, void* stream_handle, const void* ro
     const size_t slots = combine_few(route_count, token_count, top_k) ? 0u : static_cast<size_t>(token_count) * top_k;
     if (slots > sampler->combine_slots_capacity)
     {
-        // earlier calls on this stream may still use the scratch that is replaced here
-        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
-        MOE_CUDA_CHECK(sampler, grow(sampler->combine_slots, sampler->combine_slots_capacity, slots));
-        MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->combine_slots, 0, sizeof(uint32_t) * slots, stream));
+        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->combine_slots, sampler->combine_slots_capacity, slots));
+        MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->combine_slots, 0, sizeof(uint32_t) * sampler->combine_slots_capacity, stream));
     }
     args.slots = sampler->combine_slots;
     MOE_CUDA_CHECK(sampler, launch_combine_routes(args, dtype, stream));
@@ -1155,12 +1178,10 @@ int moe_balance_loss(moe_sampler* sampler, void* stream_handle, const float* rou
     DeviceGuard guard(sampler->device);
     const size_t sums = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * options->expert_count;
     const size_t counts = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * (options->expert_count + 1u);
-    if (sums > sampler->balance_sums_capacity || counts > sampler->balance_counts_capacity)
-    {
-        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
-        MOE_CUDA_CHECK(sampler, grow(sampler->balance_sums, sampler->balance_sums_capacity, sums));
-        MOE_CUDA_CHECK(sampler, grow(sampler->balance_counts, sampler->balance_counts_capacity, counts));
-    }
+    if (sums > sampler->balance_sums_capacity)
+        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->balance_sums, sampler->balance_sums_capacity, sums));
+    if (counts > sampler->balance_counts_capacity)
+        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->balance_counts, sampler->balance_counts_capacity, counts));
     args.partial_sums = sampler->balance_sums;
     args.partial_counts = sampler->balance_counts;
     MOE_CUDA_CHECK(sampler, launch_balance_loss(args, stream));

@@ -411,8 +411,8 @@ inline const char* check_quantize(const QuantizeArgs& a, int dtype, int activati
     const size_t used = static_cast<size_t>(a.columns) * (activation == MOE_ACTIVATION_SILU_GATE ? 2u : 1u);
     if (a.row_stride < used)
         return "row_stride is smaller than the columns a row uses";
-    if (a.columns > 0x7FFFFFFFu)
-        return "columns must be below 2^31";
+    if (a.columns > 0x7FFFFFFFu || a.rows > 0x7FFFFFFFu)
+        return "columns and rows must be below 2^31";
     if (a.rows == 0 || a.columns == 0)
         return nullptr;
     if ((a.source == nullptr && a.source_rows > 0) || a.values == nullptr || a.scales == nullptr)

@@ -598,6 +598,119 @@ def test_expert_layer_in_a_graph(pkg, torch_cuda):
         handle.close()
 
 
+def test_captured_graphs_outlive_larger_calls(pkg, torch_cuda):
+    """Scratch that a graph was captured with stays when a later call needs more; the larger call and the graph do not disturb each other."""
+    torch = torch_cuda
+    handle = pkg.Sampler(max_rows=1, max_vocab=64)
+    try:
+        def inputs(tokens, experts, seed):
+            plan = plan_of(torch, seed, tokens, experts, 8)
+            return plan, randn(torch, seed, tokens * 8, 48), randn(torch, seed + 1, tokens, 2048), randn(torch, seed + 2, tokens, experts)
+
+        def run(plan, rows, source, logits, out):
+            tokens = source.shape[0]
+            handle.combine_routes(rows, plan["token"], plan["rank"], plan["weight"], tokens, 8, out=out["sum"])
+            handle.quantize_rows(source, route_token=plan["token"], out=out["quantized"])
+            handle.balance_loss(logits, plan["offsets"], plan["token"], 8, out=out["balance"])
+
+        def outputs(tokens, experts):
+            return dict(sum=torch.zeros((tokens, 48), device="cuda"),
+                        quantized=(torch.zeros((tokens * 8, 2048), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((16, tokens * 8), device="cuda")),
+                        balance=pkg.BalanceLoss(torch.zeros(1, device="cuda"), torch.zeros(experts + 1, dtype=torch.int32, device="cuda"), torch.zeros(experts, device="cuda")))
+
+        small, large = inputs(600, 16, 1), inputs(2500, 200, 2)
+        out, want, other = outputs(600, 16), outputs(600, 16), outputs(2500, 200)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*small, want)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            run(*small, out)
+        first = None
+        for _ in range(3):
+            with torch.cuda.stream(side):
+                graph.replay()
+                run(*large, other)
+            side.synchronize()
+            assert torch.equal(out["sum"], want["sum"])
+            assert torch.equal(out["quantized"][0].view(torch.uint8), want["quantized"][0].view(torch.uint8)) and torch.equal(out["quantized"][1], want["quantized"][1])
+            assert torch.equal(out["balance"].loss, want["balance"].loss) and torch.equal(out["balance"].expert_tokens, want["balance"].expert_tokens)
+            now = (other["sum"].clone(), other["quantized"][0].view(torch.uint8).clone(), other["balance"].loss.clone())
+            assert first is None or all(torch.equal(a, b) for a, b in zip(first, now))
+            first = now
+            out["sum"].zero_()
+            other["sum"].zero_()
+            torch.cuda.synchronize()
+        assert handle.expert_check() == 0
+    finally:
+        handle.close()
+
+
+def test_two_handles_on_two_streams(pkg, torch_cuda):
+    torch = torch_cuda
+    handles = [pkg.Sampler(max_rows=1, max_vocab=64) for _ in range(2)]
+    try:
+        states = [layer_state(torch, pkg, tokens, 16, 4, 512, 256) for tokens in (48, 200)]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        plans = [None, None]
+        for _ in range(10):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    plans[i] = expert_layer(handles[i], pkg, *states[i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert_layer(torch, *states[i], plans[i])
+            assert handles[i].expert_check() == 0
+    finally:
+        for handle in handles:
+            handle.close()
+
+
+def test_offsets_beyond_32_bits(sampler, torch_cuda):
+    """The last rows of arrays that hold more than 2^32 values or bytes."""
+    torch = torch_cuda
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    rows, columns = 530000, 8208
+    source = torch.zeros((rows, columns), dtype=torch.bfloat16, device="cuda")
+    source[-3:] = randn(torch, 1, 3, columns).bfloat16()
+    values, scales = sampler.quantize_rows(source)
+    want_values, want_scales = quantize_reference(torch, source[-3:])
+    assert torch.equal(values[-3:].float().cpu(), want_values) and torch.equal(scales[:, -3:].cpu(), want_scales)
+    assert bool((scales[:, :-3] == 0).all())
+    # combine: the routed rows of the last tokens
+    tokens = 4
+    token = torch.full((rows,), tokens, dtype=torch.int32, device="cuda")     # out of range: left out
+    token[-3:] = torch.tensor([3, 0, 3], dtype=torch.int32, device="cuda")
+    rank = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    rank[-1] = 1
+    weight = torch.full((rows,), 0.5, device="cuda")
+    out = sampler.combine_routes(source, token, rank, weight, tokens, 2)
+    sampler.expert_check()
+    want = torch.zeros((tokens, columns), device="cuda")
+    want[3], want[0] = 0.5 * source[-3].float() + 0.5 * source[-1].float(), 0.5 * source[-2].float()
+    assert bool(((out.float() - want).abs() <= 2.0 ** -8 * want.abs() + 4 * U * source.float()[-3:].abs().sum(dim=0)).all())
+    del source, values, scales, token, rank, weight
+    # weights of more than 2^32 bytes
+    experts, outputs, columns = 70, 8192, 8208
+    weights = torch.zeros((experts, outputs, columns), dtype=torch.float8_e4m3fn, device="cuda")
+    weights[-1] = (randn(torch, 2, outputs, columns) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    weight_scales = torch.ones((experts, 64, 65), device="cuda")
+    for count in (2, 90):
+        x = (randn(torch, 3, count, columns) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+        x_scales = torch.ones((65, count), device="cuda")
+        offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+        offsets[-1] = count
+        out = sampler.expert_product(x, x_scales, weights, weight_scales, expert_offsets=offsets, out_dtype=torch.float32)
+        one = torch.tensor([0, count], dtype=torch.int32, device="cuda")
+        assert_product(torch, out, product_reference(torch, x, x_scales, weights[-1:], weight_scales[-1:], one), columns)
+    del weights
+    torch.cuda.empty_cache()
+
+
 def test_calls_follow_a_producer_that_lets_them_start_early(sampler, pkg, torch_cuda, test_kernels):
     """Inputs that the kernel before writes after it has let its successors start (see tests/test_launch_order.py)."""
     from test_launch_order import produce_late
