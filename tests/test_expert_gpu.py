@@ -214,6 +214,10 @@ def test_dense_product(sampler, torch_cuda, rows, columns, outputs, out_dtype):
 
 GROUPED = [(1, 8, 8, 256, 128), (3, 64, 4, 144, 200), (32, 128, 4, 2880, 320), (40, 16, 2, 512, 1000), (257, 8, 2, 384, 130), (130, 300, 3, 272, 72), (700, 4, 1, 1040, 264),
            (2048, 32, 4, 256, 256)]
+# several tiles of 128 rows a CTA, with one to four blocks of columns and 16 to 128 columns in the last
+GROUPED += [(4000, 4, 2, columns, 1300) for columns in (16, 128, 144, 256, 336, 512)] + [(3001, 3, 2, 384, 1000)]
+# several tiles of 16, 32 and 64 rows a CTA
+GROUPED += [(300, 80, 3, columns, 520) for columns in (32, 256, 384)] + [(600, 60, 3, 272, 520), (700, 40, 3, 144, 129), (700, 40, 3, 640, 700)]
 
 
 @pytest.mark.parametrize("tokens,experts,top_k,columns,outputs", GROUPED)
