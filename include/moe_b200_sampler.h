@@ -414,7 +414,7 @@ enum moe_activation
  *              MOE_EXPERT_FLAG_TOKEN_RANGE.
  * values       device, [rows x columns] e4m3, dense
  * scales       device, [ceil(columns / 128) x rows]: block-major
- * columns and rows < 2^31.  Asynchronous on `stream`.  Calls that route their source rows twice or more on average may
+ * columns and rows < 2^31.  Asynchronous on `stream`.  Calls that route their source rows four times or more on average may
  * quantise each row once and grow the handle's scratch for that (48 MiB at most a call); scratch grows outside of stream
  * captures, so make the largest call before one.  Graphs captured earlier stay valid. */
 int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,

@@ -305,12 +305,12 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
 // A token's routes lie in the blocks of its experts.  HBM bound: every routed row is read once, every token written once.
 // Many routes: one kernel notes for every (token, rank) the route that holds it, the next sums a token's rows with one CTA and
 // leaves the notes at zero for the next call.  Few routes: each CTA looks through all of them for those of its token, which
-// is cheaper than a second launch.  Either way a CTA first has the list of its token's routes and weights, ranks ascending, in
+// is cheaper than a second launch (128 tokens x 8 routes x 4096 3.8 against 4.9 us; 256 tokens x 4 5.5 against 4.8).  Either way a CTA first has the list of its token's routes and weights, ranks ascending, in
 // shared memory; then a thread adds 16 bytes of up to eight rows at a time.
 
 constexpr int kCombineThreads = 256;
-constexpr uint32_t kCombineFew = 4096;     // routes that every CTA looks through itself
-constexpr uint32_t kCombineFewTokens = 2048;
+constexpr uint32_t kCombineFew = 1024;     // routes that every CTA looks through itself
+constexpr uint32_t kCombineFewTokens = 128;
 constexpr uint32_t kCombineFewRanks = 64;
 
 __global__ void __launch_bounds__(256) combine_slots_kernel(const CombineArgs a)

@@ -369,15 +369,16 @@ struct BalanceArgs
 };
 // once: scratch of quantize_once_bytes for rows that are quantised once and then copied to their routes, or null
 cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, uint8_t* once, cudaStream_t stream);
-// Scratch for quantising each source row once, 0 where every route quantises its own row.  Dividing is what a call is bound by
-// (12 instructions a value), so rows with two routes or more on average gain: 4096 rows x 4096 to 32768 routes 87 us route by
-// route, %ONCE% in two passes.  The quantised rows have to stay in L2 between the passes, and are copied in 16-byte vectors; small
-// calls gain nothing from a second launch.
+// Scratch for quantising each source row once, 0 where every route quantises its own row.  Dividing costs a value three times what
+// copying a byte does, so large calls that use their rows often gain: 4096 rows x 4096 to 32768 routes 78 us route by route,
+// 45 in two passes.  To 8192 routes it costs (22 against 25 us), and so it does in small calls, by the second launch (1024 rows x
+// 4096 to 4096 routes 11.6 against 16.2; 4096 rows x 2048 to 16384 routes 21.6 against 15.8).  The quantised rows have to stay in L2 between the passes, and are copied in 16-byte
+// vectors.
 inline size_t quantize_once_bytes(const QuantizeArgs& a)
 {
     const size_t values = (static_cast<size_t>(a.source_rows) * a.columns + 15u) / 16u * 16u;
     const size_t bytes = values + sizeof(float) * a.source_rows * ((static_cast<size_t>(a.columns) + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK);
-    const bool worth = a.route_token != nullptr && a.rows / 2u >= a.source_rows && static_cast<uint64_t>(a.rows) * a.columns >= (1ull << 22);
+    const bool worth = a.route_token != nullptr && a.rows / 4u >= a.source_rows && static_cast<uint64_t>(a.rows) * a.columns >= (1ull << 25);
     const bool fits = a.columns % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 16u == 0u && a.source_rows > 0u && bytes <= (48ull << 20);
     return worth && fits ? bytes : 0u;
 }

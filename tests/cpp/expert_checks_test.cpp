@@ -52,13 +52,13 @@ int main()
         check("quantize alignment bf16", false, MOE_DTYPE_BF16, MOE_ACTIVATION_NONE, [](QuantizeArgs& a) { a.source = at<void>(258); });
     }
     {
-        // rows that are quantised once: two routes a row, 2^22 values, 16-byte vectors, scratch that stays in L2
+        // rows that are quantised once: four routes a row, 2^25 values, 16-byte vectors, scratch that stays in L2
         const auto once = [](uint32_t source_rows, uint32_t rows, uint32_t columns, size_t values) {
             const QuantizeArgs args = {at<void>(256), source_rows, rows, columns, columns, at<uint32_t>(64), at<uint8_t>(values), at<float>(64), at<uint32_t>(4)};
             return quantize_once_bytes(args);
         };
-        if (once(4096, 32768, 4096, 256) != 4096u * 4096u + 4u * 4096u * 32u || once(300, 4200, 1040, 256) != 300u * 1040u + 4u * 300u * 9u || once(4096, 8191, 4096, 256) != 0 ||
-            once(300, 4000, 1040, 256) != 0 || once(300, 4200, 1032, 256) != 0 || once(300, 4200, 1040, 264) != 0 || once(16384, 32768, 4096, 256) != 0 || once(0, 32768, 4096, 256) != 0)
+        if (once(4096, 32768, 4096, 256) != 4096u * 4096u + 4u * 4096u * 32u || once(1000, 33000, 1040, 256) != 1000u * 1040u + 4u * 1000u * 9u || once(4096, 16383, 4096, 256) != 0 ||
+            once(1000, 32000, 1040, 256) != 0 || once(1000, 33000, 1032, 256) != 0 || once(1000, 33000, 1040, 264) != 0 || once(16384, 65536, 4096, 256) != 0 || once(0, 32768, 4096, 256) != 0)
         {
             std::printf("quantize_once_bytes\n");
             ++failures;

@@ -72,9 +72,10 @@ def test_quantize_gathers(sampler, torch_cuda, dtype, columns):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("source_rows,routes,columns", [(300, 4200, 1040), (2500, 5000, 848), (7, 9000, 480), (2500, 4999, 848), (300, 4200, 1032)])
+@pytest.mark.parametrize("source_rows,routes,columns", [(1000, 33000, 1040), (2000, 16400, 2064), (7, 18000, 1872), (4200, 16799, 2064),
+                                                         (1000, 33000, 1032)])
 def test_quantize_gathers_rows_that_are_routed_often(sampler, pkg, torch_cuda, dtype, source_rows, routes, columns):
-    """Two routes a row on average, and 2^22 values: the rows are quantised once and copied (below that, or with columns that are no
+    """Four routes a row on average, and 2^25 values: the rows are quantised once and copied (below that, or with columns that are no
     multiple of 16, they are not)."""
     torch = torch_cuda
     x = (randn(torch, 5, source_rows, columns + 8) * 3).to(getattr(torch, dtype))[:, :columns]
@@ -622,8 +623,8 @@ def test_captured_graphs_outlive_larger_calls(pkg, torch_cuda):
                         quantized=(torch.zeros((tokens * 8, 2048), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((16, tokens * 8), device="cuda")),
                         balance=pkg.BalanceLoss(torch.zeros(1, device="cuda"), torch.zeros(experts + 1, dtype=torch.int32, device="cuda"), torch.zeros(experts, device="cuda")))
 
-        small, large = inputs(600, 16, 1), inputs(2500, 200, 2)
-        out, want, other = outputs(600, 16), outputs(600, 16), outputs(2500, 200)
+        small, large = inputs(2100, 16, 1), inputs(4000, 200, 2)
+        out, want, other = outputs(2100, 16), outputs(2100, 16), outputs(4000, 200)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
