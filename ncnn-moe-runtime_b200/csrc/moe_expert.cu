@@ -305,8 +305,9 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
 // A token's routes lie in the blocks of its experts.  HBM bound: every routed row is read once, every token written once.
 // Many routes: one kernel notes for every (token, rank) the route that holds it, the next sums a token's rows with one CTA and
 // leaves the notes at zero for the next call.  Few routes: each CTA looks through all of them for those of its token, which
-// is cheaper than a second launch (128 tokens x 8 routes x 4096 3.8 against 4.9 us; 256 tokens x 4 5.5 against 4.8).  Either way a CTA first has the list of its token's routes and weights, ranks ascending, in
-// shared memory; then a thread adds 16 bytes of up to eight rows at a time.
+// is cheaper than a second launch (128 tokens x 8 routes x 4096 3.8 against 4.9 us; 256 tokens x 4 5.5 against 4.8).  Either way
+// a CTA first has the list of its token's routes and weights, ranks ascending, in shared memory; then a thread adds 16 bytes of
+// up to eight rows at a time.  32768 bf16 rows x 4096 to 4096 tokens: 61 us, 5.5 TB/s, four of them for the notes.
 
 constexpr int kCombineThreads = 256;
 constexpr uint32_t kCombineFew = 1024;     // routes that every CTA looks through itself
@@ -498,8 +499,9 @@ cudaError_t launch_combine(const CombineArgs& a, cudaStream_t stream)
         return launch_following(kernel, pieces * a.token_count, kCombineThreads, 0, stream, a, pieces, piece);
     }
     const uint32_t blocks = (a.route_count + 255u) / 256u;
-    if (cudaError_t status = launch_following(combine_slots_kernel, blocks < 592u ? blocks : 592u, 256u, 0, stream, a))
-        return status;
+    if (blocks > 0u)
+        if (cudaError_t status = launch_following(combine_slots_kernel, blocks < 592u ? blocks : 592u, 256u, 0, stream, a))
+            return status;
     auto kernel = vector ? combine_routes_kernel<T, true> : combine_routes_kernel<T, false>;
     return launch_following(kernel, a.token_count < 148u * 8u ? a.token_count : 148u * 8u, kCombineThreads, sizeof(uint2) * a.top_k, stream, a);
 }

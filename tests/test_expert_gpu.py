@@ -355,6 +355,17 @@ def test_combine_partial_plans_and_strides(sampler, torch_cuda, routes_kept, tok
     assert bool(((out.double() - want).abs() <= 5 * U * size + U * want.abs()).all())
 
 
+@pytest.mark.parametrize("tokens", [5, 129, 4000])
+@pytest.mark.parametrize("top_k", [0, 4])
+def test_combine_without_routes(sampler, torch_cuda, tokens, top_k):
+    """A step whose routes were all dropped: every token gets its base, or zeros."""
+    torch = torch_cuda
+    none = torch.empty(0, dtype=torch.int32, device="cuda")
+    rows, weight, base = torch.empty((0, 72), device="cuda"), torch.empty(0, device="cuda"), randn(torch, 3, tokens, 72)
+    assert bool((sampler.combine_routes(rows, none, none, weight, tokens, top_k) == 0).all())
+    assert torch.equal(sampler.combine_routes(rows, none, none, weight, tokens, top_k, base=base), base)
+
+
 @pytest.mark.parametrize("tokens", [4, 3000])
 def test_combine_bad_and_repeated_routes(sampler, pkg, torch_cuda, tokens):
     torch = torch_cuda
