@@ -1205,10 +1205,13 @@ int moe_balance_loss_backward(moe_sampler* sampler, void* stream_handle, const f
     args.score_function = options->score_function;
     args.coefficient = coefficient;
     args.token_mask = token_mask;
+    args.expert_tokens = const_cast<uint32_t*>(expert_tokens);
     if (const char* text = check_balance(args))
         return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, text);
     if (router_logits == nullptr || expert_tokens == nullptr || logit_gradient == nullptr)
         return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, "balance buffers must not be null");
+    if (misaligned(loss_gradient, 4u) || misaligned(logit_gradient, 4u))
+        return fail(sampler, MOE_STATUS_INVALID_ARGUMENT, "balance buffers must be aligned to their elements");
     DeviceGuard guard(sampler->device);
     MOE_CUDA_CHECK(sampler, launch_balance_loss_backward(args, expert_tokens, loss_gradient, logit_gradient, static_cast<cudaStream_t>(stream_handle)));
     return MOE_STATUS_OK;

@@ -473,6 +473,9 @@ inline const char* check_balance(const BalanceArgs& a)
         return "score_function must be a moe_router_score";
     if (!(a.coefficient - a.coefficient == 0.0f))
         return "the balance coefficient must be finite";
+    if (misaligned(a.logits, 4u) || misaligned(a.expert_offsets, 4u) || misaligned(a.route_token, 4u) || misaligned(a.expert_tokens, 4u) ||
+        misaligned(a.expert_probability, 4u) || misaligned(a.loss, 4u))
+        return "balance buffers must be aligned to their elements";
     return nullptr;
 }
 

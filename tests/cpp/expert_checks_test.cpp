@@ -114,6 +114,12 @@ int main()
     {
         BalanceArgs args = {};
         expect("balance", check_balance(args), false);
+        args.logits = at<float>(66);
+        expect("balance logits alignment", check_balance(args), true);
+        args.logits = at<float>(64);
+        args.expert_tokens = at<uint32_t>(65);
+        expect("balance tokens alignment", check_balance(args), true);
+        args.expert_tokens = nullptr;
         args.score_function = 3;
         expect("balance score", check_balance(args), true);
         args.score_function = MOE_ROUTER_SQRT_SOFTPLUS;
