@@ -472,7 +472,7 @@ int moe_expert_check(moe_sampler* sampler, void* stream, uint32_t* flags);
  * scores of a token divided by their sum over the experts (softmax rows already sum to 1), n the tokens
  * that count, c_e the routes of those tokens that went to expert e, E experts and k routes a token:
  *   P_e = sum of p_e over the tokens / n,   loss = coefficient * sum over e of (E * c_e / (k * n)) * P_e
- * A token whose scores are all zero counts, with p = 0.  With n = 0 all results are 0.  Non-finite logits
+ * A token whose scores are all zero in fp32 counts, with p = 0.  With n = 0 all results are 0.  Non-finite logits
  * (which moe_router_dispatch refuses) give what the arithmetic gives.
  *
  * router_logits   device, [token_count x expert_count], as for moe_router_dispatch

@@ -36,6 +36,16 @@ __device__ __forceinline__ float warp_sum(float v)
         v += __shfl_xor_sync(kFullMask, v, offset);
     return v;
 }
+// two sums side by side
+__device__ __forceinline__ void warp_sum_both(float& v, float& w)
+{
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1)
+    {
+        v += __shfl_xor_sync(kFullMask, v, offset);
+        w += __shfl_xor_sync(kFullMask, w, offset);
+    }
+}
 __device__ __forceinline__ float warp_max(float v)
 {
 #pragma unroll
@@ -115,6 +125,31 @@ struct LaneRow
 __device__ __forceinline__ float factor_of(float total)
 {
     return total == 0.0f ? 0.0f : __fdiv_rn(1.0f, total);
+}
+
+// Scores that sum to less than this are tiny for all experts: sigmoid is exp(x) there, sqrt-softplus exp(x / 2), to all digits.
+// They may be subnormal and the reciprocal of their sum infinite, so a token with such a sum (not zero: those count as zeros) is
+// taken again relative to its largest logit, as softmax is.
+constexpr float kTinyScores = 0x1p-60f;
+__device__ __forceinline__ bool tiny_scores(float total)
+{
+    return total > 0.0f && total < kTinyScores;
+}
+template<int kFunction>
+__device__ __forceinline__ float tiny_score(float x, float peak)
+{
+    return expf((kFunction == MOE_ROUTER_SQRT_SOFTPLUS ? 0.5f : 1.0f) * (x - peak));
+}
+// a tiny score's derivative over the score
+template<int kFunction>
+constexpr float kTinySlope = kFunction == MOE_ROUTER_SQRT_SOFTPLUS ? 0.5f : 1.0f;
+// the largest of a token's logits; a warp
+__device__ __forceinline__ float largest_logit(const float* logits, uint32_t experts)
+{
+    float peak = -INFINITY;
+    for (uint32_t e = threadIdx.x & 31u; e < experts; e += 32u)
+        peak = fmaxf(peak, logits[e]);
+    return warp_max(peak);
 }
 
 // ---- forward ------------------------------------------------------------------------------
@@ -275,7 +310,21 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(cons
                     x[i] = 0.0f;
                 total += x[i];
             }
-            const float factor = factor_of(warp_sum(total));
+            total = warp_sum(total);
+            if (kFunction != MOE_ROUTER_SOFTMAX && tiny_scores(total))
+            {
+                const float* logits = a.logits + token * experts;
+                peak = largest_logit(logits, experts);
+                total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                {
+                    x[i] = lane + 32u * i < experts ? tiny_score<kFunction>(logits[lane + 32u * i], peak) : 0.0f;
+                    total += x[i];
+                }
+                total = warp_sum(total);
+            }
+            const float factor = factor_of(total);
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
                 sum[i] = fmaf(x[i], factor, sum[i]);
@@ -296,13 +345,7 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(cons
                 continue;
             ++counted;
             const float* logits = a.logits + token * experts;
-            float peak = -INFINITY;
-            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
-            {
-                for (uint32_t e = lane; e < experts; e += 32u)
-                    peak = fmaxf(peak, logits[e]);
-                peak = warp_max(peak);
-            }
+            float peak = kFunction == MOE_ROUTER_SOFTMAX ? largest_logit(logits, experts) : 0.0f;
             float total = 0.0f;
             for (uint32_t e = lane; e < experts; e += 32u)
             {
@@ -311,7 +354,19 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_partial_kernel(cons
                 row[e] = score;
                 total += score;
             }
-            const float factor = factor_of(warp_sum(total));
+            total = warp_sum(total);
+            if (kFunction != MOE_ROUTER_SOFTMAX && tiny_scores(total))
+            {
+                peak = largest_logit(logits, experts);
+                total = 0.0f;
+                for (uint32_t e = lane; e < experts; e += 32u)
+                {
+                    row[e] = tiny_score<kFunction>(logits[e], peak);
+                    total += row[e];
+                }
+                total = warp_sum(total);
+            }
+            const float factor = factor_of(total);
             for (uint32_t e = lane; e < experts; e += 32u)
                 sum_row[e] = fmaf(row[e], factor, sum_row[e]);
         }
@@ -480,11 +535,21 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(con
                 total += score;
                 mean = fmaf(share[i], score, mean);
             }
-#pragma unroll
-            for (int offset = 16; offset > 0; offset >>= 1) // two sums side by side
+            warp_sum_both(total, mean);
+            if (kFunction != MOE_ROUTER_SOFTMAX && tiny_scores(total))
             {
-                total += __shfl_xor_sync(kFullMask, total, offset);
-                mean += __shfl_xor_sync(kFullMask, mean, offset);
+                const float* logits = a.logits + token * experts;
+                peak = largest_logit(logits, experts);
+                total = mean = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                {
+                    const float score = lane + 32u * i < experts ? tiny_score<kFunction>(logits[lane + 32u * i], peak) : 0.0f;
+                    slope[i] = kTinySlope<kFunction> * score;
+                    total += score;
+                    mean = fmaf(share[i], score, mean);
+                }
+                warp_sum_both(total, mean);
             }
             const float factor = factor_of(total);
             mean *= factor;
@@ -506,13 +571,7 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(con
                 continue;
             }
             const float* logits = a.logits + token * experts;
-            float peak = -INFINITY;
-            if constexpr (kFunction == MOE_ROUTER_SOFTMAX)
-            {
-                for (uint32_t e = lane; e < experts; e += 32u)
-                    peak = fmaxf(peak, logits[e]);
-                peak = warp_max(peak);
-            }
+            float peak = kFunction == MOE_ROUTER_SOFTMAX ? largest_logit(logits, experts) : 0.0f;
             float total = 0.0f, mean = 0.0f;
             for (uint32_t e = lane; e < experts; e += 32u)
             {
@@ -521,12 +580,28 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(con
                 total += score;
                 mean = fmaf(shares[e], score, mean);
             }
-            const float factor = factor_of(warp_sum(total));
-            mean = warp_sum(mean) * factor;
+            warp_sum_both(total, mean);
+            const bool tiny = kFunction != MOE_ROUTER_SOFTMAX && tiny_scores(total);
+            if (tiny)
+            {
+                peak = largest_logit(logits, experts);
+                total = mean = 0.0f;
+                for (uint32_t e = lane; e < experts; e += 32u)
+                {
+                    const float score = tiny_score<kFunction>(logits[e], peak);
+                    total += score;
+                    mean = fmaf(shares[e], score, mean);
+                }
+                warp_sum_both(total, mean);
+            }
+            const float factor = factor_of(total);
+            mean *= factor;
             for (uint32_t e = lane; e < experts; e += 32u)
             {
                 float score, slope;
                 score_of<kFunction, true>(logits[e], peak, score, slope);
+                if (tiny)
+                    slope = kTinySlope<kFunction> * tiny_score<kFunction>(logits[e], peak);
                 target[e] = factor == 0.0f ? 0.0f : slope * factor * (shares[e] - mean);
             }
         }

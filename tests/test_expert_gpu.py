@@ -508,6 +508,28 @@ def test_balance_without_tokens_and_with_dead_rows(sampler, pkg, torch_cuda):
         assert bool((gradient[5] == 0).all()) and bool(torch.isfinite(gradient).all())
 
 
+@pytest.mark.parametrize("score,tops", [("sigmoid", (-42.0, -80.0, -89.0, -95.0, -102.0)), ("sqrtsoftplus", (-84.0, -160.0, -176.0, -190.0, -204.0))])
+@pytest.mark.parametrize("experts", [24, 256, 1000, 1500])
+def test_balance_of_tiny_scores(sampler, pkg, torch_cuda, score, tops, experts):
+    """Tokens whose scores are tiny or subnormal for every expert, down to where the largest is about to become zero.  Bounds as in
+    test_balance, and 256 units more: the rounding of x - peak (at most 2^-24 of 256) is a score's relative error."""
+    torch = torch_cuda
+    logits = 1.5 * randn(torch, 21, 40, experts)
+    for row, top in enumerate(tops):
+        logits[row] += top - logits[row].max()
+        logits[row + 8] = top       # all equal
+    logits[20, 1:] = tops[1]        # one expert far above the others
+    plan = plan_of(torch, 8, 40, experts, 3)
+    counts, n, mean, loss, gradient, size = balance_reference(torch, logits, plan, 3, score, None, 0.01, 1.0)
+    out = sampler.balance_loss(logits, plan["offsets"], plan["token"], 3, score_function=score_code(pkg, score), coefficient=0.01)
+    rel = (experts + 40 + 16 + 256) * U
+    assert bool(((out.expert_probability.double() - mean).abs() <= rel * mean + 1e-40).all())
+    assert abs(float(out.loss) - loss) <= (rel + (experts + 8) * U) * abs(loss)
+    got = sampler.balance_loss_backward(logits, out.expert_tokens, 3, score_function=score_code(pkg, score), coefficient=0.01)
+    bound = (2 * experts + 32 + 512) * U * size + 1e-40
+    assert bool(((got.double() - gradient).abs() <= bound).all()), float(((got.double() - gradient).abs() / bound).max())
+
+
 def test_balance_does_not_follow_bad_plans(sampler, pkg, torch_cuda):
     torch = torch_cuda
     logits = randn(torch, 2, 30, 8)
