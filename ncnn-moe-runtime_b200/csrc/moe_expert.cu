@@ -71,14 +71,13 @@ struct Eight
 // ---- quantisation -------------------------------------------------------------------
 //
 // scale = max |x| / 448 over a block of 128 columns, value = e4m3(x / scale).  Sixteen lanes own a block, eight values each, so
-// that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row and has all their loads in flight before the
-// first maximum.  Bound by instructions before memory (three quarters of the issue slots), so what belongs to a block is done
-// once for the four blocks of a half warp: their maxima are reduced side by side until a lane has one of them, and it divides
-// and inverts that one.
+// that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row (small calls: 256) and has all their loads in
+// flight before the first maximum.  Large calls are bound by instructions before memory (16384 gated bf16 rows x 4096: 86 us, 71 %
+// of the issue slots, 3.9 TB/s), so what belongs to a block is done once for the four blocks of a half warp: their maxima are
+// reduced side by side until a lane has one of them, and it divides and inverts that one.
 
 constexpr int kQuantizeThreads = 128;
-constexpr int kQuantizeSteps = 4;                               // blocks of 128 a half warp takes from one item
-constexpr uint32_t kQuantizeItem = 256u * kQuantizeSteps;       // columns of an item
+constexpr uint32_t kQuantizeItem = 256u; // columns of an item, by its steps: the blocks of 128 that a half warp takes from it
 constexpr float kE4m3Max = 448.0f;
 
 __device__ __forceinline__ uint32_t to_e4m3_pair(float low, float high)
@@ -134,19 +133,21 @@ __device__ __forceinline__ float reduce_blocks(const float (&top)[4], uint32_t s
     return fmaxf(c, __shfl_xor_sync(kFullMask, c, 1));
 }
 
-template<typename T, bool kGate, bool kVector>
+template<typename T, bool kGate, bool kVector, int kSteps>
 __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const QuantizeArgs a)
 {
+    if (a.release_next)
+        grid_dependency_release();
     wait_for_previous_kernel();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t half = lane >> 4, sub = lane & 15u;
-    const uint32_t pieces = (a.columns + kQuantizeItem - 1u) / kQuantizeItem;
+    const uint32_t pieces = (a.columns + kQuantizeItem * kSteps - 1u) / (kQuantizeItem * kSteps);
     const uint64_t items = static_cast<uint64_t>(a.rows) * pieces;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (kQuantizeThreads / 32);
     for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kQuantizeThreads / 32) + (threadIdx.x >> 5); item < items; item += stride)
     {
         const uint32_t row = static_cast<uint32_t>(item / pieces);
-        const uint32_t first = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * pieces) * kQuantizeItem;
+        const uint32_t first = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * pieces) * (kQuantizeItem * kSteps);
         uint32_t source_row = row;
         bool valid = true;
         if (a.route_token != nullptr)
@@ -157,10 +158,10 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
                 atomicOr(a.flags, MOE_EXPERT_FLAG_TOKEN_RANGE);
         }
         const T* source = static_cast<const T*>(a.source) + static_cast<size_t>(valid ? source_row : 0u) * a.row_stride;
-        Eight<T> gate[kQuantizeSteps];
-        Eight<T> up[kGate ? kQuantizeSteps : 1];
+        Eight<T> gate[kSteps];
+        Eight<T> up[kGate ? kSteps : 1];
 #pragma unroll
-        for (int s = 0; s < kQuantizeSteps; ++s)
+        for (int s = 0; s < kSteps; ++s)
         {
             const uint32_t column = first + 256u * s + 128u * half + 8u * sub;
             const uint32_t count = valid && column < a.columns ? min(8u, a.columns - column) : 0u;
@@ -182,10 +183,10 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
                     up[s].load_scalars(source + a.columns + column, count);
             }
         }
-        float x[kQuantizeSteps][8];
-        float top[kQuantizeSteps];
+        float x[kSteps][8];
+        float top[kSteps];
 #pragma unroll
-        for (int s = 0; s < kQuantizeSteps; ++s)
+        for (int s = 0; s < kSteps; ++s)
         {
             gate[s].unpack(x[s]);
             if constexpr (kGate)
@@ -201,11 +202,25 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
             for (int i = 0; i < 8; ++i)
                 top[s] = fmaxf(top[s], fabsf(x[s][i]));
         }
-        static_assert(kQuantizeSteps == 4, "a lane divides for one block of four");
-        const float scale = __fdiv_rn(reduce_blocks(top, sub), kE4m3Max);
+        // the block that this lane divides for: all of its half warp's lanes for the one, or four lanes for each of four
+        static_assert(kSteps == 1 || kSteps == 4, "a lane divides for one block");
+        float largest;
+        if constexpr (kSteps == 4)
         {
-            const uint32_t block_begin = first + 256u * (sub >> 2) + 128u * half; // the block that this lane divides for
-            if ((sub & 3u) == 0u && block_begin < a.columns)
+            largest = reduce_blocks(top, sub);
+        }
+        else
+        {
+            largest = top[0];
+#pragma unroll
+            for (int offset = 8; offset > 0; offset >>= 1)
+                largest = fmaxf(largest, __shfl_xor_sync(kFullMask, largest, offset));
+        }
+        constexpr uint32_t kSharers = 16u / kSteps;
+        const float scale = __fdiv_rn(largest, kE4m3Max);
+        {
+            const uint32_t block_begin = first + 256u * (sub / kSharers) + 128u * half;
+            if (sub % kSharers == 0u && block_begin < a.columns)
                 a.scales[static_cast<size_t>(block_begin / MOE_EXPERT_BLOCK) * a.rows + row] = scale;
         }
         // A block of zeros, or one whose scale underflows, is divided by one: zeros, and NaN where there is one.
@@ -215,10 +230,10 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
         // remainders are exact as above; a dividend too small for that gives a quotient far below e4m3's smallest.)
         const bool short_way = __all_sync(kFullMask, scale == 0.0f || (scale >= 0x1p-24f && scale < 0x1p25f && correction_decides(scale)));
 #pragma unroll
-        for (int s = 0; s < kQuantizeSteps; ++s)
+        for (int s = 0; s < kSteps; ++s)
         {
             const uint32_t column = first + 256u * s + 128u * half + 8u * sub;
-            const float by = __shfl_sync(kFullMask, divisor, 16u * half + 4u * s), inverse = __shfl_sync(kFullMask, reciprocal, 16u * half + 4u * s);
+            const float by = __shfl_sync(kFullMask, divisor, 16u * half + kSharers * s), inverse = __shfl_sync(kFullMask, reciprocal, 16u * half + kSharers * s);
             if (short_way)
             {
 #pragma unroll
@@ -247,7 +262,9 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
 }
 
 // Rows that were quantised once, copied to every route that names them: a byte a value from L2 and to HBM.  A warp copies a row,
-// 4 KiB in flight; the scales, which lie block by block, follow in a loop of their own.
+// 4 KiB in flight, and marks what it writes as not to be kept in L2, where the rows are that it reads (4096 rows x 4096 to 32768
+// routes: both passes 35 us, 45 without the mark; the product behind it gains too, 132 -> 127 us for both calls).  The scales,
+// which lie block by block, follow in a loop of their own.
 constexpr int kSpreadThreads = 256;
 __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const QuantizeArgs a, const uint8_t* values, const float* scales)
 {
@@ -272,7 +289,7 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const Quant
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i)
                 if (first + 32u * i < vectors)
-                    target[first + 32u * i] = part[i];
+                    __stcs(&target[first + 32u * i], part[i]);
         }
     }
     const uint32_t blocks = (a.columns + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK;
@@ -287,17 +304,27 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const Quant
     }
 }
 
-template<typename T>
-cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t stream)
+template<typename T, int kSteps>
+cudaError_t launch_quantize_steps(const QuantizeArgs& a, bool gate, cudaStream_t stream)
 {
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.source);
     const bool vector = a.columns % 8u == 0u && bases % 16u == 0u && a.row_stride * sizeof(T) % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 8u == 0u;
-    const uint64_t items = static_cast<uint64_t>(a.rows) * ((a.columns + kQuantizeItem - 1u) / kQuantizeItem);
+    const uint64_t items = static_cast<uint64_t>(a.rows) * ((a.columns + kQuantizeItem * kSteps - 1u) / (kQuantizeItem * kSteps));
     const uint64_t blocks = (items + kQuantizeThreads / 32 - 1) / (kQuantizeThreads / 32);
     const uint32_t grid = static_cast<uint32_t>(blocks < 148u * 16u ? blocks : 148u * 16u);
-    auto kernel = gate ? (vector ? quantize_rows_kernel<T, true, true> : quantize_rows_kernel<T, true, false>)
-                       : (vector ? quantize_rows_kernel<T, false, true> : quantize_rows_kernel<T, false, false>);
+    auto kernel = gate ? (vector ? quantize_rows_kernel<T, true, true, kSteps> : quantize_rows_kernel<T, true, false, kSteps>)
+                       : (vector ? quantize_rows_kernel<T, false, true, kSteps> : quantize_rows_kernel<T, false, false, kSteps>);
     return launch_following(kernel, grid, kQuantizeThreads, 0, stream, a);
+}
+// Small calls wait for one item's latency, so they are cut finer: 128 x 2880 fp32 gated 2.6 us with one step, 4.1 with four; 256 x
+// 4096 bf16 2.3 against 2.8, 1024 x 4096 gated 7.2 against 7.7.  Above, the divisions that four blocks share pay: 512 x 4096 3.3
+// against 3.5, 2048 x 4096 gated 12.5 against 13.9, 4096 x 4096 11.3 against 15.4.
+template<typename T>
+cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t stream)
+{
+    if (static_cast<uint64_t>(a.rows) * a.columns <= (gate ? 1ull << 22 : 1ull << 20))
+        return launch_quantize_steps<T, 1>(a, gate, stream);
+    return launch_quantize_steps<T, 4>(a, gate, stream);
 }
 
 // ---- combine --------------------------------------------------------------------------
@@ -307,7 +334,8 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
 // leaves the notes at zero for the next call.  Few routes: each CTA looks through all of them for those of its token, which
 // is cheaper than a second launch (128 tokens x 8 routes x 4096 3.8 against 4.9 us; 256 tokens x 4 5.5 against 4.8).  Either way
 // a CTA first has the list of its token's routes and weights, ranks ascending, in shared memory; then a thread adds 16 bytes of
-// up to eight rows at a time.  32768 bf16 rows x 4096 to 4096 tokens: 61 us, 5.5 TB/s, four of them for the notes.
+// up to eight rows at a time; rows are read once and marked so.  32768 bf16 rows x 4096 to 4096 tokens: 52 us (6.4 TB/s), without
+// the mark 56.
 
 constexpr int kCombineThreads = 256;
 constexpr uint32_t kCombineFew = 1024;     // routes that every CTA looks through itself
@@ -316,6 +344,7 @@ constexpr uint32_t kCombineFewRanks = 64;
 
 __global__ void __launch_bounds__(256) combine_slots_kernel(const CombineArgs a)
 {
+    grid_dependency_release(); // the kernel that sums is on the SMs, waiting, when this one ends
     wait_for_previous_kernel();
     for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < a.route_count; i += static_cast<uint64_t>(gridDim.x) * blockDim.x)
     {
@@ -397,7 +426,7 @@ __device__ __forceinline__ void sum_token(const CombineArgs& a, uint32_t token, 
 #pragma unroll
             for (uint32_t i = 0; i < kRows; ++i)
                 if (first + i < count)
-                    part[i] = *reinterpret_cast<const Load*>(rows + static_cast<size_t>(list[first + i].x) * a.row_stride + column);
+                    part[i] = __ldcs(reinterpret_cast<const Load*>(rows + static_cast<size_t>(list[first + i].x) * a.row_stride + column));
 #pragma unroll
             for (uint32_t i = 0; i < kRows; ++i)
                 if (first + i < count)
@@ -516,6 +545,7 @@ cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activa
         // every source row once, then a copy for each route
         QuantizeArgs rows = args;
         rows.route_token = nullptr;
+        rows.release_next = true;
         rows.rows = args.source_rows;
         rows.values = once;
         rows.scales = reinterpret_cast<float*>(once + (static_cast<size_t>(args.source_rows) * args.columns + 15u) / 16u * 16u);
@@ -523,7 +553,7 @@ cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activa
         if (status != cudaSuccess)
             return status;
         const uint32_t blocks = (args.rows + kSpreadThreads / 32 - 1) / (kSpreadThreads / 32);
-        return launch_following(spread_rows_kernel, blocks < 148u * 8u ? blocks : 148u * 8u, kSpreadThreads, 0, stream, args, rows.values, rows.scales);
+        return launch_following(spread_rows_kernel, blocks < 148u * 32u ? blocks : 148u * 32u, kSpreadThreads, 0, stream, args, rows.values, rows.scales);
     }
     return dtype == MOE_DTYPE_F32 ? launch_quantize<float>(args, gate, stream) : launch_quantize<__nv_bfloat16>(args, gate, stream);
 }

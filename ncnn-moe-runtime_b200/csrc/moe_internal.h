@@ -314,6 +314,8 @@ struct QuantizeArgs
     uint8_t* values;
     float* scales;
     uint32_t* flags; // MOE_EXPERT_FLAG_* of the handle
+    // the call's second kernel follows and may take its places on the SMs while the first one runs
+    bool release_next = false;
 };
 struct ProductArgs
 {
@@ -371,9 +373,9 @@ struct BalanceArgs
 cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activation, uint8_t* once, cudaStream_t stream);
 // Scratch for quantising each source row once, 0 where every route quantises its own row.  Dividing costs a value three times what
 // copying a byte does, so large calls that use their rows often gain: 4096 rows x 4096 to 32768 routes 78 us route by route,
-// 45 in two passes.  To 8192 routes it costs (22 against 25 us), and so it does in small calls, by the second launch (1024 rows x
-// 4096 to 4096 routes 11.6 against 16.2; 4096 rows x 2048 to 16384 routes 21.6 against 15.8).  The quantised rows have to stay in L2 between the passes, and are copied in 16-byte
-// vectors.
+// 35 in two passes; 4096 rows x 2048 to 16384 routes 21.6 against 15.8.  To 8192 routes it costs (22 against 25 us), and so it does
+// in small calls, by the second launch (1024 rows x 4096 to 4096 routes 11.6 against 16.2).  The quantised rows have to stay in L2
+// between the passes, and are copied in 16-byte vectors.
 inline size_t quantize_once_bytes(const QuantizeArgs& a)
 {
     const size_t values = (static_cast<size_t>(a.source_rows) * a.columns + 15u) / 16u * 16u;

@@ -131,6 +131,32 @@ def test_quantize_special_values(sampler, torch_cuda):
     assert bool((values[7, :128] == 448).all())
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,columns", [(5000, 1032), (4300, 999), (1100, 4104), (34000, 130)])
+def test_quantize_large_calls_are_their_parts(sampler, pkg, torch_cuda, dtype, gated, rows, columns):
+    """Small and large calls divide the work differently and must agree bit for bit, special values included; ungated rows also
+    with the plain formula."""
+    torch = torch_cuda
+    activation = pkg.ACTIVATION_SILU_GATE if gated else pkg.ACTIVATION_NONE
+    x = randn(torch, 4, rows, columns * (2 if gated else 1)).to(getattr(torch, dtype))
+    x[7] = 0
+    x[9, 3] = float("nan")
+    x[rows - 2, -1] = float("inf")
+    x[11] *= 1e-38
+    x[12] *= 1e30
+    x[13, : columns // 2] = 448.0
+    values, scales = sampler.quantize_rows(x, activation=activation)
+    for first in range(0, rows, 100):
+        part, part_scales = sampler.quantize_rows(x[first:first + 100], activation=activation)
+        assert torch.equal(part.view(torch.uint8), values[first:first + 100].view(torch.uint8))
+        assert torch.equal(part_scales, scales[:, first:first + 100])
+    if not gated:
+        plain = [row for row in range(rows) if row not in (9, rows - 2)]
+        want_values, want_scales = quantize_reference(torch, x[plain])
+        assert torch.equal(scales.cpu()[:, plain], want_scales) and torch.equal(values.float().cpu()[plain], want_values)
+
+
 def test_quantize_refuses_to_follow_a_bad_route(sampler, pkg, torch_cuda):
     torch = torch_cuda
     x = randn(torch, 3, 4, 300)
