@@ -11,6 +11,7 @@ The directory name is not a Python identifier; load it with
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -198,6 +199,12 @@ def _value_dtype(tensor, name):
     if dtype is torch.bfloat16:
         return DTYPE_BF16
     raise TypeError(f"{name} must be float32 or bfloat16")
+
+
+@functools.lru_cache(maxsize=64)
+def _balance_options(experts, top_k, score_function):
+    """The options that the balance calls look at (read-only there)."""
+    return RouterOptions(experts, top_k, score_function, 0, 1.0, 0, None, None)
 
 
 def _address(tensor, name, shape, dtype, device):
@@ -561,11 +568,14 @@ class Sampler:
         rows = source_rows if route_token is None else route_token.numel()
         blocks = (columns + EXPERT_BLOCK - 1) // EXPERT_BLOCK
         if out is None:
-            out = (torch.empty(rows, columns, dtype=torch.float8_e4m3fn, device=source.device), torch.empty(blocks, rows, dtype=torch.float32, device=source.device))
-        values, scales = out
+            values = torch.empty(rows, columns, dtype=torch.float8_e4m3fn, device=source.device)
+            scales = torch.empty(blocks, rows, dtype=torch.float32, device=source.device)
+            values_address, scales_address = values.data_ptr(), scales.data_ptr()
+        else:
+            values, scales = out
+            values_address = _address(values, "values", (rows, columns), torch.float8_e4m3fn, device)
+            scales_address = _address(scales, "scales", (blocks, rows), torch.float32, device)
         routes = _address(route_token, "route_token", (rows,), torch.int32, device)
-        values_address = _address(values, "values", (rows, columns), torch.float8_e4m3fn, device)
-        scales_address = _address(scales, "scales", (blocks, rows), torch.float32, device)
         if rows == 0:
             return values, scales
         self._check(self._lib.moe_quantize_rows(self._handle, self._stream(stream), address, dtype, source_rows, columns, source.stride(0) if source_rows > 1 else width,
@@ -605,11 +615,14 @@ class Sampler:
         routes, columns = route_rows.shape
         if out is None:
             out = torch.empty(token_count, columns, dtype=route_rows.dtype, device=route_rows.device)
+            out_address = out.data_ptr()
+        else:
+            out_address = _address(out, "out", (token_count, columns), route_rows.dtype, device)
         self._check(self._lib.moe_combine_routes(
             self._handle, self._stream(stream), address, dtype, route_rows.stride(0) if routes > 1 else columns, columns,
             _address(route_token, "route_token", (routes,), torch.int32, device), _address(route_rank, "route_rank", (routes,), torch.int32, device),
             _address(route_weight, "route_weight", (routes,), torch.float32, device), routes, token_count, top_k,
-            _address(base, "base", (token_count, columns), route_rows.dtype, device), _address(out, "out", (token_count, columns), route_rows.dtype, device)))
+            _address(base, "base", (token_count, columns), route_rows.dtype, device), out_address))
         return out
 
     def expert_check(self, stream=None) -> int:
@@ -629,12 +642,15 @@ class Sampler:
             place = router_logits.device
             out = BalanceLoss(torch.empty(1, dtype=torch.float32, device=place), torch.empty(experts + 1, dtype=torch.int32, device=place),
                               torch.empty(experts, dtype=torch.float32, device=place))
-        options = RouterOptions(experts, top_k, score_function, 0, 1.0, 0, None, None)
+            results = out.expert_tokens.data_ptr(), out.expert_probability.data_ptr(), out.loss.data_ptr()
+        else:
+            results = (_address(out.expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
+                       _address(out.expert_probability, "expert_probability", (experts,), torch.float32, device), _address(out.loss, "loss", (1,), torch.float32, device))
+        options = _balance_options(experts, top_k, score_function)
         self._check(self._lib.moe_balance_loss(
             self._handle, self._stream(stream), _address(router_logits, "router_logits", (tokens, experts), torch.float32, device), tokens, C.byref(options),
             _address(expert_offsets, "expert_offsets", (experts + 1,), torch.int32, device), _address(route_token, "route_token", (tokens * top_k,), torch.int32, device),
-            self._mask_address(token_mask, tokens), coefficient, _address(out.expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
-            _address(out.expert_probability, "expert_probability", (experts,), torch.float32, device), _address(out.loss, "loss", (1,), torch.float32, device)))
+            self._mask_address(token_mask, tokens), coefficient, *results))
         return out
 
     def _mask_address(self, token_mask, tokens):
@@ -652,9 +668,12 @@ class Sampler:
         tokens, experts = router_logits.shape
         if out is None:
             out = torch.empty(tokens, experts, dtype=torch.float32, device=router_logits.device)
-        options = RouterOptions(experts, top_k, score_function, 0, 1.0, 0, None, None)
+            out_address = out.data_ptr()
+        else:
+            out_address = _address(out, "out", (tokens, experts), torch.float32, device)
+        options = _balance_options(experts, top_k, score_function)
         self._check(self._lib.moe_balance_loss_backward(
             self._handle, self._stream(stream), _address(router_logits, "router_logits", (tokens, experts), torch.float32, device), tokens, C.byref(options),
             self._mask_address(token_mask, tokens), coefficient, _address(expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
-            _address(loss_gradient, "loss_gradient", (1,), torch.float32, device), _address(out, "out", (tokens, experts), torch.float32, device)))
+            _address(loss_gradient, "loss_gradient", (1,), torch.float32, device), out_address))
         return out
