@@ -313,6 +313,22 @@ def test_product_strides_and_one_expert_of_many(sampler, torch_cuda):
     assert bool((store[:, :5] == 0).all()) and bool((store[:, 269:] == 0).all())
 
 
+@pytest.mark.parametrize("out_dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("outputs,width,first", [(4096, 4096, 0), (4096, 4112, 16), (4104, 4128, 8), (4112, 4120, 0), (4112, 4112, 0), (4101, 4200, 32), (4096, 4097, 1), (4100, 4104, 4),
+                                                 (4240, 4256, 0)])
+def test_product_of_many_rows_into_any_place(sampler, torch_cuda, outputs, width, first, out_dtype):
+    """Tiles of 128 rows, filled and partly filled, into outputs of every alignment; nothing else is written."""
+    torch = torch_cuda
+    rows, cuts = 1500, [3, 700, 701, 1490]
+    inputs = product_inputs(torch, 5, rows, 144, 3, outputs)
+    offsets = torch.tensor(cuts, dtype=torch.int32, device="cuda")
+    store = torch.full((rows, width), -7.0, dtype=getattr(torch, out_dtype), device="cuda")
+    out = sampler.expert_product(*inputs, expert_offsets=offsets, out=store[:, first:first + outputs])
+    total, size = product_reference(torch, *inputs, offsets)
+    assert_product(torch, out[3:1490], (total[3:1490], size[3:1490]), 144)
+    assert bool((store[:3] == -7).all()) and bool((store[1490:] == -7).all()) and bool((store[:, :first] == -7).all()) and bool((store[:, first + outputs:] == -7).all())
+
+
 def test_product_refusals(sampler, pkg, torch_cuda):
     torch = torch_cuda
     values, scales, weights, weight_scales = product_inputs(torch, 2, 8, 256, 2, 64)
