@@ -334,7 +334,7 @@ cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t strea
 // leaves the notes at zero for the next call.  Few routes: each CTA looks through all of them for those of its token, which
 // is cheaper than a second launch (128 tokens x 8 routes x 4096 3.8 against 4.9 us; 256 tokens x 4 5.5 against 4.8).  Either way
 // a CTA first has the list of its token's routes and weights, ranks ascending, in shared memory; then a thread adds 16 bytes of
-// up to eight rows at a time; rows are read once and marked so.  32768 bf16 rows x 4096 to 4096 tokens: 52 us (6.4 TB/s), without
+// up to eight rows at a time; rows are read once and marked so.  32768 bf16 rows x 4096 to 4096 tokens: 52 us (5.8 TB/s), without
 // the mark 56.
 
 constexpr int kCombineThreads = 256;
