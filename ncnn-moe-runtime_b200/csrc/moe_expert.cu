@@ -136,8 +136,6 @@ __device__ __forceinline__ float reduce_blocks(const float (&top)[4], uint32_t s
 template<typename T, bool kGate, bool kVector, int kSteps>
 __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const QuantizeArgs a)
 {
-    if (a.release_next)
-        grid_dependency_release();
     wait_for_previous_kernel();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t half = lane >> 4, sub = lane & 15u;
@@ -183,6 +181,7 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
                     up[s].load_scalars(source + a.columns + column, count);
             }
         }
+        grid_dependency_release(); // the next kernel may take its places on the SMs, behind these loads
         float x[kSteps][8];
         float top[kSteps];
 #pragma unroll
@@ -545,7 +544,6 @@ cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activa
         // every source row once, then a copy for each route
         QuantizeArgs rows = args;
         rows.route_token = nullptr;
-        rows.release_next = true;
         rows.rows = args.source_rows;
         rows.values = once;
         rows.scales = reinterpret_cast<float*>(once + (static_cast<size_t>(args.source_rows) * args.columns + 15u) / 16u * 16u);

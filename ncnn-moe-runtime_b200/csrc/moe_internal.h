@@ -314,8 +314,6 @@ struct QuantizeArgs
     uint8_t* values;
     float* scales;
     uint32_t* flags; // MOE_EXPERT_FLAG_* of the handle
-    // the call's second kernel follows and may take its places on the SMs while the first one runs
-    bool release_next = false;
 };
 struct ProductArgs
 {
