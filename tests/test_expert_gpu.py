@@ -728,6 +728,29 @@ def test_captured_graphs_outlive_larger_calls(pkg, torch_cuda):
         handle.close()
 
 
+def test_layer_behind_a_refused_dispatch(sampler, pkg, torch_cuda):
+    """Plan arrays that no dispatch has filled: every call stays inside its buffers, and the check says that something was wrong."""
+    torch = torch_cuda
+    generator = torch.Generator(device="cuda").manual_seed(9)
+    tokens, experts, top_k, columns, outputs = 300, 8, 4, 256, 384
+    routes = tokens * top_k
+    x = randn(torch, 1, tokens, columns)
+    weights = (randn(torch, 2, experts, outputs, columns) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    weight_scales = torch.ones((experts, blocks_of(outputs), blocks_of(columns)), device="cuda")
+    for low, high in ((-2 ** 31, 2 ** 31 - 1), (0, 2 * tokens), (0, 2 * routes)):
+        offsets, token, rank = (torch.randint(low, high, (n,), generator=generator, device="cuda").int() for n in (experts + 1, routes, routes))
+        store = torch.full((routes + 16, outputs), -7.0, device="cuda")
+        total_store = torch.full((tokens + 16, outputs), -7.0, device="cuda")
+        values, scales = sampler.quantize_rows(x, route_token=token)
+        sampler.expert_product(values, scales, weights, weight_scales, expert_offsets=offsets, out=store[8:-8])
+        sampler.combine_routes(store[8:-8], token, rank, torch.ones(routes, device="cuda"), tokens, top_k, out=total_store[8:-8])
+        out = sampler.balance_loss(randn(torch, 3, tokens, experts), offsets, token, top_k)
+        assert sampler.expert_check() == pkg.EXPERT_FLAG_TOKEN_RANGE | pkg.EXPERT_FLAG_OFFSETS
+        assert int(out.expert_tokens[:-1].sum()) == 0
+        for part in (store[:8], store[-8:], total_store[:8], total_store[-8:], store[8:-8]):
+            assert bool((part == -7).all())    # the product did not follow such offsets
+
+
 def test_two_handles_on_two_streams(pkg, torch_cuda):
     torch = torch_cuda
     handles = [pkg.Sampler(max_rows=1, max_vocab=64) for _ in range(2)]
