@@ -536,7 +536,9 @@ struct ManyShape
     static constexpr uint32_t kColumns = kTileOutputs / 2u; // outputs that a warp sums: one block of the weights' scales
     static constexpr uint32_t kChunk = 32;
     static constexpr uint32_t kBarriers = 2u * kStages + 2u * kAccumulators;
-    static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kBarriers * 8u + 64u;
+    static constexpr uint32_t kTurnStride = 17; // words of a row that a warp turns around, one of them so that columns lie in different banks
+    static constexpr uint32_t kTurnBytes = 32u * kTurnStride * 4u;
+    static constexpr uint32_t kFixedBytes = kStages * kStageBytes + kBarriers * 8u + kSumWarps * kTurnBytes + 64u;
     // 128 sums in a thread: the warps that sum take registers over from the other roles.  Launched with 168 a thread:
     // 128 * 40 + 256 * 232 = 384 * 168.
     static constexpr uint32_t kRoleRegisters = 40;
@@ -583,7 +585,12 @@ __device__ __forceinline__ void exchange_of_four(uint32_t (&words)[4][8], uint32
     }
 }
 
+// Outputs that a lane stores at once as one vector, or two of 16 bytes.
 template<typename Out>
+constexpr uint32_t kStoreVector = 32u / sizeof(Out);
+
+// Rows of outputs start and end at multiples of kAlignment bytes: 32, 16, or (1) anywhere.
+template<typename Out, uint32_t kAlignment>
 __global__ void __launch_bounds__(ManyShape::kThreads, 1)
     expert_product_many_kernel(const ProductArgs a, const __grid_constant__ CUtensorMap weight_map, const __grid_constant__ CUtensorMap row_map)
 {
@@ -598,7 +605,7 @@ __global__ void __launch_bounds__(ManyShape::kThreads, 1)
     rings.empty = rings.full + 8u * S::kStages;
     rings.sum_full = rings.empty + 8u * S::kStages;
     rings.sum_empty = rings.sum_full + 8u * S::kAccumulators;
-    uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + 8u * S::kBarriers);
+    uint32_t* const first_tile = reinterpret_cast<uint32_t*>(shared + S::kStages * S::kStageBytes + 8u * S::kBarriers + S::kSumWarps * S::kTurnBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     if (threadIdx.x == 0)
@@ -784,13 +791,12 @@ __global__ void __launch_bounds__(ManyShape::kThreads, 1)
             const uint32_t output = tile.output_tile * kTileOutputs + half * S::kColumns;
             if (idle || output >= a.outputs)
                 continue;
-            // Whole lines of 128 bytes: four lanes exchange what they have of four rows, and each stores 32 bytes of every one of
-            // them, since the stores of all CTAs fall together.  4096 x 4096 x 4096 to bf16 74.7 us, each lane 32 bytes of its own
-            // row 76.2, without storing 68.4; to fp32 79.0 and 84.7.
-            constexpr uint32_t kVector = 32u / sizeof(Out);
+            // Whole lines of 128 bytes, since the stores of all CTAs fall together: four lanes exchange what they have of four rows, and
+            // each stores 32 bytes of every one of them.  4096 x 4096 x 4096 to bf16 74 us, each lane 32 bytes of its own row 76,
+            // without storing 68; to fp32 80 and 85.
+            constexpr uint32_t kVector = kStoreVector<Out>;
             const uint32_t count = min(S::kColumns, a.outputs - output);
-            const uint32_t alignment = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(a.out) | (a.out_stride * sizeof(Out))) % 32u;
-            if (alignment == 0u && count % kVector == 0u)
+            if constexpr (kAlignment >= 16u)
             {
                 const uint32_t first_row = quarter * 32u + (lane & ~3u);
                 Out* const target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + first_row) * a.out_stride + output + (lane & 3u) * kVector;
@@ -812,36 +818,63 @@ __global__ void __launch_bounds__(ManyShape::kThreads, 1)
                     for (uint32_t r = 0; r < 4u; ++r)
                     {
                         const uint32_t(&w)[8] = words[r];
-                        if (first_row + r < tile.rows && i + (lane & 3u) * kVector < count)
-                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(target + r * a.out_stride + i), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                                         "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                        const uint32_t column = i + (lane & 3u) * kVector;
+                        Out* const place = target + r * a.out_stride + i;
+                        if (first_row + r >= tile.rows || column >= count)
+                            continue;
+                        if constexpr (kAlignment == 32u)
+                        {
+                            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(place), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                                         "r"(w[6]), "r"(w[7])
                                          : "memory");
+                        }
+                        else
+                        {
+                            *reinterpret_cast<uint4*>(place) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (column + kVector <= count)
+                                *reinterpret_cast<uint4*>(place + kVector / 2u) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
                     }
                 }
             }
-            else if (row < tile.rows)
+            else
             {
-                Out* const target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + row) * a.out_stride + output;
+                // Rows that start anywhere: the warp turns 64 bytes of its 32 rows around in shared memory and stores neighbouring
+                // outputs side by side (4096 x 4096 x 4095 to bf16 92 us, each
+                // lane those of its row 234; 128 experts of 120 rows x 768 x 2467 to fp32 114 and 268).
+                constexpr uint32_t kPass = 64u / sizeof(Out);   // outputs
+                constexpr uint32_t kAtOnce = 32u / kPass;       // rows
+                unsigned char* const turn = shared + S::kStages * S::kStageBytes + 8u * S::kBarriers + (warp - 4u) * S::kTurnBytes;
+                const uint32_t column = lane % kPass;
+                const uint32_t end = min(32u, tile.rows - quarter * 32u);
+                Out* const target = static_cast<Out*>(a.out) + static_cast<size_t>(tile.first_row + quarter * 32u) * a.out_stride + output + column;
 #pragma unroll
-                for (uint32_t i = 0; i < S::kColumns; i += kVector)
+                for (uint32_t i = 0; i < S::kColumns; i += kPass)
                 {
-                    float values[kVector];
+                    if (i >= count)
+                        break;
+                    uint32_t words[2][8];
 #pragma unroll
-                    for (uint32_t j = 0; j < kVector; ++j)
-                        values[j] = sums[i + j];
-                    if (alignment % 16u == 0u && i + kVector <= count)
+                    for (uint32_t v = 0; v < 2u; ++v)
                     {
-                        uint32_t w[8];
-                        pack_outputs(w, values);
-                        reinterpret_cast<uint4*>(target + i)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                        reinterpret_cast<uint4*>(target + i)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
-                    else
-                    {
+                        float values[kVector];
 #pragma unroll
                         for (uint32_t j = 0; j < kVector; ++j)
-                            if (i + j < count)
-                                store_output(target + i + j, values[j]);
+                            values[j] = sums[i + v * kVector + j];
+                        pack_outputs(words[v], values);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16u; ++j)
+                        reinterpret_cast<uint32_t*>(turn)[lane * S::kTurnStride + j] = words[j / 8u][j % 8u];
+                    __syncwarp();
+#pragma unroll 8
+                    for (uint32_t first = 0; first < end; first += kAtOnce)
+                    {
+                        const uint32_t r = first + lane / kPass;
+                        const Out value = reinterpret_cast<const Out*>(turn + r * S::kTurnStride * 4u)[column];
+                        if (r < end && i + column < count)
+                            target[static_cast<size_t>(r) * a.out_stride + i] = value;
                     }
                 }
             }
@@ -930,13 +963,13 @@ cudaError_t launch_few(const ProductArgs& a, int sm_count, cudaStream_t stream)
         split *= 2u;
     return launch_tiles(expert_product_few_kernel<kTokens, Out>, opt_in, a, kTokens, kLanes, (tiles < most ? tiles * split : most), split, S::kThreads, S::kFixedBytes, stream, split);
 }
-template<typename Out>
+template<typename Out, uint32_t kAlignment>
 cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
     using S = ManyShape;
     static SharedOptIn opt_in;
     const uint64_t tiles = most_tiles(a, kLanes, kTileOutputs), most = static_cast<uint64_t>(sm_count);
-    return launch_tiles(expert_product_many_kernel<Out>, opt_in, a, kLanes, kTileOutputs, tiles < most ? tiles : most, 1u, S::kThreads, S::kFixedBytes, stream);
+    return launch_tiles(expert_product_many_kernel<Out, kAlignment>, opt_in, a, kLanes, kTileOutputs, tiles < most ? tiles : most, 1u, S::kThreads, S::kFixedBytes, stream);
 }
 
 // Experts are taken to have equal numbers of rows.  Up to 32 a tile of as many rows wastes least (64 experts of 32 rows x
@@ -958,7 +991,10 @@ cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stre
     };
     if (waves(64u, kLanes) * 3u <= waves(kLanes, kTileOutputs) * 5u)
         return launch_few<64, Out>(a, sm_count, stream);
-    return launch_many<Out>(a, sm_count, stream);
+    const uint64_t places = reinterpret_cast<uintptr_t>(a.out) | a.out_stride * sizeof(Out) | a.outputs * sizeof(Out);
+    if (places % 32u == 0u)
+        return launch_many<Out, 32u>(a, sm_count, stream);
+    return places % 16u == 0u ? launch_many<Out, 16u>(a, sm_count, stream) : launch_many<Out, 1u>(a, sm_count, stream);
 }
 
 } // namespace
