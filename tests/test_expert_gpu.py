@@ -329,6 +329,21 @@ def test_product_of_many_rows_into_any_place(sampler, torch_cuda, outputs, width
     assert bool((store[:3] == -7).all()) and bool((store[1490:] == -7).all()) and bool((store[:, :first] == -7).all()) and bool((store[:, first + outputs:] == -7).all())
 
 
+@pytest.mark.parametrize("rows_each,outputs", [(1, 130), (40, 200), (40, 201), (66, 129)])
+def test_product_of_the_most_experts(sampler, pkg, torch_cuda, rows_each, outputs):
+    torch = torch_cuda
+    experts = pkg.EXPERT_MAX_EXPERTS
+    inputs = product_inputs(torch, 6, rows_each * experts, 32, experts, outputs)
+    offsets = rows_each * torch.arange(experts + 1, dtype=torch.int32, device="cuda")
+    out = sampler.expert_product(*inputs, expert_offsets=offsets, out_dtype=torch.float32)
+    values, scales, weights, weight_scales = inputs
+    for e in (0, 1, 77, experts - 2, experts - 1):
+        mine = slice(e * rows_each, (e + 1) * rows_each)
+        part = (values[mine], scales[:, mine].contiguous(), weights[e:e + 1], weight_scales[e:e + 1])
+        assert_product(torch, out[mine], product_reference(torch, *part, None), 32)
+    assert sampler.expert_check() == 0
+
+
 def test_product_refusals(sampler, pkg, torch_cuda):
     torch = torch_cuda
     values, scales, weights, weight_scales = product_inputs(torch, 2, 8, 256, 2, 64)
