@@ -450,9 +450,10 @@ int moe_expert_product(moe_sampler* sampler, void* stream, const uint8_t* values
  *              MOE_EXPERT_FLAG_TOKEN_RANGE; of several routes with the same token and rank the last counts.
  * base         device, [token_count x columns] of dtype, or NULL; may be `out`
  * out          device, [token_count x columns] of dtype, not overlapping route_rows; a token without routes gets its base, or zeros
- * top_k <= MOE_EXPERT_MAX_EXPERTS.  Asynchronous on `stream`.  Calls with more routes than any before on this handle grow its scratch
- * (token_count * top_k words) outside of stream captures; make the largest one before a capture.  Graphs captured earlier
- * stay valid. */
+ * top_k <= MOE_EXPERT_MAX_EXPERTS.  Asynchronous on `stream`.  Calls of more than 1024 routes, 128 tokens or top 64 take scratch of
+ * token_count * top_k words.  It grows, at least twofold where there is memory for that, and what it replaces is kept until the handle
+ * goes, so graphs captured earlier stay valid.  A call that would have to grow it inside a stream capture, of whatever mode, is refused
+ * with MOE_STATUS_CUDA_ERROR and the capture goes on: make the largest one before. */
 int moe_combine_routes(moe_sampler* sampler, void* stream, const void* route_rows, int dtype, size_t row_stride, uint32_t columns,
                        const uint32_t* route_token, const uint32_t* route_rank, const float* route_weight, uint32_t route_count, uint32_t token_count,
                        uint32_t top_k, const void* base, void* out);
@@ -486,7 +487,7 @@ int moe_expert_check(moe_sampler* sampler, void* stream, uint32_t* flags);
  * expert_probability  device, [expert_count]: P_e
  * loss            device, one float
  * Sums have a fixed order: equal inputs give equal bits.  Asynchronous on `stream`; the first call on a handle, and
- * one with more experts than any before, allocates scratch: make it before a stream capture. */
+ * one with more experts than any before, allocates scratch: make it before a stream capture, where it is refused. */
 int moe_balance_loss(moe_sampler* sampler, void* stream, const float* router_logits, uint32_t token_count, const moe_router_options* options,
                      const uint32_t* expert_offsets, const uint32_t* route_token, const uint8_t* token_mask, float coefficient, uint32_t* expert_tokens,
                      float* expert_probability, float* loss);

@@ -144,30 +144,14 @@ cudaError_t grow(T*& pointer, size_t& capacity, size_t wanted)
     return status;
 }
 
-// Scratch of calls that may be captured: what a captured graph was given stays allocated until the handle goes, so a later,
-// larger call does not take it away.  At least doubled each time, so all of it together stays below twice the largest.
+// grow_kept for an entry point: a moe_status, with the text of what went wrong.
 template<typename T>
-cudaError_t grow_kept(std::vector<void*>& kept, T*& pointer, size_t& capacity, size_t wanted)
+int grow_scratch(moe_sampler* sampler, T*& pointer, size_t& capacity, size_t wanted, cudaStream_t stream, bool cleared)
 {
-    const size_t entries = wanted > 2u * capacity ? wanted : 2u * capacity;
-    try
-    {
-        kept.reserve(kept.size() + 1u); // no exception may leave a C entry point
-    }
-    catch (const std::bad_alloc&)
-    {
-        return cudaErrorMemoryAllocation;
-    }
-    T* larger = nullptr;
-    cudaError_t status = cudaMalloc(reinterpret_cast<void**>(&larger), entries * sizeof(T));
-    if (status == cudaSuccess)
-    {
-        if (pointer != nullptr)
-            kept.push_back(pointer);
-        pointer = larger;
-        capacity = entries;
-    }
-    return status;
+    const cudaError_t status = grow_kept(sampler->kept_scratch, pointer, capacity, wanted, stream, cleared);
+    if (status == cudaErrorStreamCaptureUnsupported)
+        return fail(sampler, MOE_STATUS_CUDA_ERROR, "scratch does not grow inside a stream capture: make the largest call before it");
+    return status == cudaSuccess ? MOE_STATUS_OK : fail_cuda(sampler, status, "scratch");
 }
 
 struct DeviceGuard
@@ -1099,8 +1083,9 @@ int moe_quantize_rows(moe_sampler* sampler, void* stream_handle, const void* sou
     DeviceGuard guard(sampler->device);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     const size_t once = quantize_once_bytes(args);
-    if (once > sampler->quantize_once_capacity)
-        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->quantize_once, sampler->quantize_once_capacity, once));
+    if (once > 0)
+        if (int status = grow_scratch(sampler, sampler->quantize_once, sampler->quantize_once_capacity, once, stream, false))
+            return status;
     MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, once > 0 ? sampler->quantize_once : nullptr, stream));
     return MOE_STATUS_OK;
 }
@@ -1135,13 +1120,16 @@ int moe_combine_routes(moe_sampler* sampler, void* stream_handle, const void* ro
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     DeviceGuard guard(sampler->device);
     const size_t slots = combine_few(route_count, token_count, top_k) ? 0u : static_cast<size_t>(token_count) * top_k;
-    if (slots > sampler->combine_slots_capacity)
-    {
-        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->combine_slots, sampler->combine_slots_capacity, slots));
-        MOE_CUDA_CHECK(sampler, cudaMemsetAsync(sampler->combine_slots, 0, sizeof(uint32_t) * sampler->combine_slots_capacity, stream));
-    }
+    if (int status = grow_scratch(sampler, sampler->combine_slots, sampler->combine_slots_capacity, slots, stream, true))
+        return status;
     args.slots = sampler->combine_slots;
-    MOE_CUDA_CHECK(sampler, launch_combine_routes(args, dtype, stream));
+    const cudaError_t launched = launch_combine_routes(args, dtype, stream);
+    if (launched != cudaSuccess)
+    {
+        // the notes that the first of two launches may have left are not cleared: the next call takes other slots
+        sampler->combine_slots_capacity = 0;
+        return fail_cuda(sampler, launched, "combine");
+    }
     return MOE_STATUS_OK;
 }
 
@@ -1178,10 +1166,10 @@ int moe_balance_loss(moe_sampler* sampler, void* stream_handle, const float* rou
     DeviceGuard guard(sampler->device);
     const size_t sums = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * options->expert_count;
     const size_t counts = static_cast<size_t>(MOE_BALANCE_MAX_BLOCKS) * (options->expert_count + 1u);
-    if (sums > sampler->balance_sums_capacity)
-        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->balance_sums, sampler->balance_sums_capacity, sums));
-    if (counts > sampler->balance_counts_capacity)
-        MOE_CUDA_CHECK(sampler, grow_kept(sampler->kept_scratch, sampler->balance_counts, sampler->balance_counts_capacity, counts));
+    if (int status = grow_scratch(sampler, sampler->balance_sums, sampler->balance_sums_capacity, sums, stream, false))
+        return status;
+    if (int status = grow_scratch(sampler, sampler->balance_counts, sampler->balance_counts_capacity, counts, stream, false))
+        return status;
     args.partial_sums = sampler->balance_sums;
     args.partial_counts = sampler->balance_counts;
     MOE_CUDA_CHECK(sampler, launch_balance_loss(args, stream));

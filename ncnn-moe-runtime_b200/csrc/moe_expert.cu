@@ -435,8 +435,8 @@ __device__ __forceinline__ void sum_token(const CombineArgs& a, uint32_t token, 
     }
 }
 
-// Packs the routes noted in slots[0 .. top_k) (0: none), which may be global or shared memory, with their weights.  One warp;
-// returns their number.
+// Packs the routes noted in slots[0 .. top_k) (0: none), which may be global or shared memory, with their weights.  A note that is
+// no route of the call is not followed.  One warp; returns their number.
 __device__ __forceinline__ uint32_t list_routes(const CombineArgs& a, const uint32_t* slots, uint2* list)
 {
     const uint32_t lane = threadIdx.x & 31u;
@@ -444,8 +444,9 @@ __device__ __forceinline__ uint32_t list_routes(const CombineArgs& a, const uint
     for (uint32_t first = 0; first < a.top_k; first += 32u)
     {
         const uint32_t slot = first + lane < a.top_k ? slots[first + lane] : 0u;
-        const unsigned taken = __ballot_sync(kFullMask, slot != 0u);
-        if (slot != 0u)
+        const bool noted = slot - 1u < a.route_count;
+        const unsigned taken = __ballot_sync(kFullMask, noted);
+        if (noted)
             list[count + __popc(taken & ((1u << lane) - 1u))] = make_uint2(slot - 1u, __float_as_uint(a.route_weight[slot - 1u]));
         count += __popc(taken);
     }

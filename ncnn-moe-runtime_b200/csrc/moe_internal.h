@@ -5,7 +5,9 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <new>
 #include <string>
+#include <vector>
 
 #include "../../include/moe_b200_sampler.h"
 
@@ -268,6 +270,58 @@ ClusterOccupancy cluster_occupancy(ClusterOccupancyTable& table, int device, Que
         table.known[device] = true;
     }
     return found;
+}
+
+// Scratch of calls that may be captured: what a captured graph was given stays allocated (in `kept`) until the handle goes, so
+// a later, larger call does not take it away.  At least doubled each time where there is memory for that, so all of it together
+// stays below twice the largest.  Nothing grows inside a capture: in the relaxed mode the allocation would succeed there, but a
+// clearing would only be recorded, and a call before the first replay would find whatever the memory held.  pointer and capacity
+// change only behind a clearing that was enqueued.
+template<typename T>
+cudaError_t grow_kept(std::vector<void*>& kept, T*& pointer, size_t& capacity, size_t wanted, cudaStream_t stream, bool cleared)
+{
+    if (wanted <= capacity)
+        return cudaSuccess;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaError_t status = cudaStreamIsCapturing(stream, &capturing))
+        return status;
+    if (capturing != cudaStreamCaptureStatusNone)
+        return cudaErrorStreamCaptureUnsupported;
+    try
+    {
+        kept.reserve(kept.size() + 1u); // no exception may leave a C entry point
+    }
+    catch (const std::bad_alloc&)
+    {
+        return cudaErrorMemoryAllocation;
+    }
+    void* larger = nullptr;
+    size_t entries = wanted > 2u * capacity ? wanted : 2u * capacity;
+    cudaError_t status = cudaMalloc(&larger, entries * sizeof(T));
+    if (status == cudaErrorMemoryAllocation && entries > wanted)
+    {
+        entries = wanted;
+        status = cudaMalloc(&larger, entries * sizeof(T));
+    }
+    if (status != cudaSuccess)
+    {
+        (void)cudaGetLastError(); // it is reported here, not by the caller's next launch
+        return status;
+    }
+    if (cleared)
+    {
+        status = cudaMemsetAsync(larger, 0, entries * sizeof(T), stream);
+        if (status != cudaSuccess)
+        {
+            cudaFree(larger);
+            return status;
+        }
+    }
+    if (pointer != nullptr)
+        kept.push_back(pointer);
+    pointer = static_cast<T*>(larger);
+    capacity = entries;
+    return cudaSuccess;
 }
 
 // All kernels but the router's three launches (and the reset before them in moe_router_dispatch_static) are launched while
