@@ -415,8 +415,8 @@ enum moe_activation
  * values       device, [rows x columns] e4m3, dense
  * scales       device, [ceil(columns / 128) x rows]: block-major
  * columns and rows < 2^31.  Asynchronous on `stream`.  Calls that route their source rows four times or more on average may
- * quantise each row once and grow the handle's scratch for that (48 MiB at most a call); scratch grows outside of stream
- * captures, so make the largest call before one.  Graphs captured earlier stay valid. */
+ * quantise each row once, in scratch of 48 MiB that the first of them on a handle allocates outside of a stream capture; where
+ * there is none yet inside a capture, or no memory for it, every route quantises its own row: slower, the same bits. */
 int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, int dtype, uint32_t source_rows, uint32_t columns, size_t row_stride,
                       int activation, const uint32_t* route_token, uint32_t route_count, uint8_t* values, float* scales);
 

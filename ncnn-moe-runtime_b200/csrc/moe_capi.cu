@@ -74,7 +74,7 @@ struct moe_sampler
     int32_t* gather_status = nullptr;        // one word: set when moe_regroup_gather met a token index out of range
     // expert products and balance
     uint32_t* expert_flags = nullptr;  // one word: MOE_EXPERT_FLAG_* met since the last check
-    uint8_t* quantize_once = nullptr;  // rows that are quantised once and copied to their routes
+    uint8_t* quantize_once = nullptr;  // kQuantizeOnceBytes: rows that are quantised once and copied to their routes
     size_t quantize_once_capacity = 0;
     uint32_t* combine_slots = nullptr; // zeros between calls
     size_t combine_slots_capacity = 0;
@@ -1082,11 +1082,16 @@ int moe_quantize_rows(moe_sampler* sampler, void* stream_handle, const void* sou
         return MOE_STATUS_OK;
     DeviceGuard guard(sampler->device);
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
-    const size_t once = quantize_once_bytes(args);
-    if (once > 0)
-        if (int status = grow_scratch(sampler, sampler->quantize_once, sampler->quantize_once_capacity, once, stream, false))
-            return status;
-    MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, once > 0 ? sampler->quantize_once : nullptr, stream));
+    bool once = quantize_once_bytes(args) > 0;
+    if (once)
+    {
+        const cudaError_t status = grow_kept(sampler->kept_scratch, sampler->quantize_once, sampler->quantize_once_capacity, kQuantizeOnceBytes, stream, false);
+        // without memory for it, or inside a capture, each route quantises its own row, to the same bits
+        once = status == cudaSuccess;
+        if (!once && status != cudaErrorMemoryAllocation && status != cudaErrorStreamCaptureUnsupported)
+            return fail_cuda(sampler, status, "scratch");
+    }
+    MOE_CUDA_CHECK(sampler, launch_quantize_rows(args, dtype, activation, once ? sampler->quantize_once : nullptr, stream));
     return MOE_STATUS_OK;
 }
 

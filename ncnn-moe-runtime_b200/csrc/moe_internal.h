@@ -428,12 +428,13 @@ cudaError_t launch_quantize_rows(const QuantizeArgs& args, int dtype, int activa
 // 35 in two passes; 4096 rows x 2048 to 16384 routes 21.6 against 15.8.  To 8192 routes it costs (22 against 25 us), and so it does
 // in small calls, by the second launch (1024 rows x 4096 to 4096 routes 11.6 against 16.2).  The quantised rows have to stay in L2
 // between the passes, and are copied in 16-byte vectors.
+constexpr size_t kQuantizeOnceBytes = 48u << 20; // the most, and what a handle allocates at its first such call
 inline size_t quantize_once_bytes(const QuantizeArgs& a)
 {
     const size_t values = (static_cast<size_t>(a.source_rows) * a.columns + 15u) / 16u * 16u;
     const size_t bytes = values + sizeof(float) * a.source_rows * ((static_cast<size_t>(a.columns) + MOE_EXPERT_BLOCK - 1u) / MOE_EXPERT_BLOCK);
     const bool worth = a.route_token != nullptr && a.rows / 4u >= a.source_rows && static_cast<uint64_t>(a.rows) * a.columns >= (1ull << 25);
-    const bool fits = a.columns % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 16u == 0u && a.source_rows > 0u && bytes <= (48ull << 20);
+    const bool fits = a.columns % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 16u == 0u && a.source_rows > 0u && bytes <= kQuantizeOnceBytes;
     return worth && fits ? bytes : 0u;
 }
 // whether a combine needs no slots: each of its CTAs looks through the routes

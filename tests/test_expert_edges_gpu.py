@@ -69,3 +69,49 @@ def test_balance_refuses_to_grow_inside_a_capture(pkg, torch_cuda):
         assert torch.equal(place.loss, want.loss) and torch.equal(place.expert_probability, want.expert_probability)
     finally:
         handle.close()
+
+
+def often_routed(torch, source_rows, columns):
+    """Rows that are quantised once and copied: 4.5 routes a row, 2^25 values and more."""
+    routes = source_rows * 9 // 2
+    source = randn(torch, 7, source_rows, columns).bfloat16()
+    index = torch.randint(source_rows, (routes,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").int()
+    blocks = (columns + 127) // 128
+    out = (torch.zeros((routes, columns), dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros((blocks, routes), device="cuda"))
+    return source, index, out
+
+
+def test_quantize_scratch_is_bounded(pkg, torch_cuda):
+    """Whatever calls a handle has seen, it holds 48 MiB for rows that are quantised once (allocations come in 2 MiB)."""
+    torch = torch_cuda
+    handle = pkg.Sampler(max_rows=1, max_vocab=64)
+    try:
+        calls = [often_routed(torch, rows, 4096) for rows in (2500, 6200, 6500, 11500)]
+        handle.quantize_rows(calls[0][0][:8])
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        for source, index, out in calls:
+            handle.quantize_rows(source, route_token=index, out=out)
+        torch.cuda.synchronize()
+        assert before - torch.cuda.mem_get_info()[0] <= 50 << 20
+    finally:
+        handle.close()
+
+
+def test_quantize_captured_before_any_scratch(pkg, torch_cuda):
+    """Captured as the handle's first call: the bits of the call that quantises each row once."""
+    torch = torch_cuda
+    source, index, out = often_routed(torch, 2500, 4096)
+    handle = pkg.Sampler(max_rows=1, max_vocab=64)
+    try:
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            handle.quantize_rows(source, route_token=index, out=out)
+        graph.replay()
+        torch.cuda.synchronize()
+        values, scales = handle.quantize_rows(source, route_token=index)
+        assert torch.equal(values.view(torch.uint8), out[0].view(torch.uint8)) and torch.equal(scales, out[1])
+    finally:
+        handle.close()
