@@ -591,7 +591,7 @@ __global__ void __launch_bounds__(kThreadsFor<kPer>) balance_backward_kernel(con
                 float score, slope;
                 slope_of<kFunction>(logits[e], peak, score, slope);
                 if (tiny)
-                    slope = kTinySlope<kFunction> * tiny_score<kFunction>(logits[e], peak);
+                    slope = zero_scores<kFunction>(peak) ? 0.0f : kTinySlope<kFunction> * tiny_score<kFunction>(logits[e], peak);
                 target[e] = slope * factor * (shares[e] - mean);
             }
         }

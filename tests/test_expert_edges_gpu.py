@@ -1,7 +1,7 @@
 """Edges of the expert calls on the GPU: scratch and stream captures.  Helpers and the rule for tolerances: tests/test_expert_gpu.py."""
 import pytest
 
-from test_expert_gpu import U, combine_reference, plan_of, randn
+from test_expert_gpu import U, combine_reference, plan_of, randn, score_code
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,28 @@ def test_quantize_captured_before_any_scratch(pkg, torch_cuda):
         assert torch.equal(values.view(torch.uint8), out[0].view(torch.uint8)) and torch.equal(scales, out[1])
     finally:
         handle.close()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "sqrtsoftplus"])
+@pytest.mark.parametrize("experts", [24, 256, 1000, 1500])
+@pytest.mark.parametrize("lowest", [float("-inf"), -3.4028234663852886e38])
+def test_balance_of_tokens_masked_for_every_expert(sampler, pkg, torch_cuda, score, experts, lowest):
+    """Scores that are zeros: the token counts with probabilities 0 and has gradient 0.  One expert left: gradient 0 for the others."""
+    torch = torch_cuda
+    tokens, code = 20, score_code(pkg, score)
+    logits = 1.5 * randn(torch, 31, tokens, experts)
+    plan = plan_of(torch, 8, tokens, experts, 3)
+    logits[4] = lowest
+    logits[9, 1:] = lowest
+    out = sampler.balance_loss(logits, plan["offsets"], plan["token"], 3, score_function=code)
+    rest = logits.clone()
+    rest[4] = 0
+    mask = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    mask[4] = False
+    without = sampler.balance_loss(rest, plan["offsets"], plan["token"], 3, score_function=code, token_mask=mask)
+    want = without.expert_probability.double() * (tokens - 1) / tokens
+    # the same sums in another order over at most 20 tokens, and a division each
+    assert bool(((out.expert_probability.double() - want).abs() <= 24 * U * want).all()) and int(out.expert_tokens[-1]) == tokens
+    gradient = sampler.balance_loss_backward(logits, out.expert_tokens, 3, score_function=code)
+    assert bool((gradient[4] == 0).all()) and bool(torch.isfinite(gradient).all())
+    assert bool((gradient[9, 1:] == 0).all())
