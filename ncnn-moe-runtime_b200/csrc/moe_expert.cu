@@ -72,8 +72,8 @@ struct Eight
 //
 // scale = max |x| / 448 over a block of 128 columns, value = e4m3(x / scale).  Sixteen lanes own a block, eight values each, so
 // that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row (small calls: 256) and has all their loads in
-// flight before the first maximum.  Large calls are bound by instructions before memory (16384 gated bf16 rows x 4096: 86 us, 71 %
-// of the issue slots, 3.9 TB/s), so what belongs to a block is done once for the four blocks of a half warp: their maxima are
+// flight before the first maximum.  Large calls are bound by instructions before memory (16384 gated bf16 rows x 4096: 82 us,
+// 4.1 TB/s), so what belongs to a block is done once for the four blocks of a half warp: their maxima are
 // reduced side by side until a lane has one of them, and it divides and inverts that one.
 
 constexpr int kQuantizeThreads = 128;
@@ -101,13 +101,26 @@ __device__ __forceinline__ float divide_once(float a, float b, float r)
     return __fmaf_rn(__fmaf_rn(-q, b, a), r, q);
 }
 
+// gate / below * up where the short way below does not hold: infinities and NaN, and gates from -41 down.  From -88.7 down the
+// denominator has left fp32, and the quotient is gate * exp(gate): in two halves.  Apart, since inlined it costs the common way a third.
+__device__ __noinline__ float silu_gate_apart(float gate, float below, float up)
+{
+    if (gate < 0.0f && below == INFINITY)
+    {
+        const float half = expf(0.5f * gate);
+        return gate * half * up * half;
+    }
+    return __fmul_rn(__fdiv_rn(gate, below), up);
+}
+
 // gate / (1 + exp(-gate)) * up; the quotient within a unit in the last place
 __device__ __forceinline__ float silu_gate(float gate, float up)
 {
     const float below = 1.0f + expf(-gate);
     // (from 2^126 on the reciprocal leaves the normal numbers; an infinity has no remainder)
-    const float quotient = below < 0x1p60f && gate < INFINITY ? divide_once(gate, below, approximate_reciprocal(below)) : __fdiv_rn(gate, below);
-    return __fmul_rn(quotient, up);
+    if (below < 0x1p60f && gate < INFINITY)
+        return __fmul_rn(divide_once(gate, below, approximate_reciprocal(below)), up);
+    return silu_gate_apart(gate, below, up);
 }
 
 // Whether one correction decides e4m3's rounding as the correctly rounded quotient does.  They differ only where the quotient
@@ -133,8 +146,12 @@ __device__ __forceinline__ float reduce_blocks(const float (&top)[4], uint32_t s
     return fmaxf(c, __shfl_xor_sync(kFullMask, c, 1));
 }
 
+// Large gated calls of bf16 rows keep eight blocks on an SM (64 registers; 16384 rows x 4096 82 us, with the seven of 71 registers 90).
+template<typename T, bool kGate, int kSteps>
+constexpr int kQuantizeBlocks = kGate && sizeof(T) == 2u && kSteps == 4 ? 8 : 0;
+
 template<typename T, bool kGate, bool kVector, int kSteps>
-__global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const QuantizeArgs a)
+__global__ void __launch_bounds__(kQuantizeThreads, kQuantizeBlocks<T, kGate, kSteps>) quantize_rows_kernel(const QuantizeArgs a)
 {
     wait_for_previous_kernel();
     const uint32_t lane = threadIdx.x & 31u;

@@ -117,6 +117,40 @@ def test_quantize_captured_before_any_scratch(pkg, torch_cuda):
         handle.close()
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,columns", [(64, 300), (5000, 1032)])
+def test_quantize_gate_far_below_zero(sampler, pkg, torch_cuda, dtype, rows, columns):
+    """Gates whose exp(-gate) is beyond fp32 and ups that bring the product back: h = gate * e * up * e with e = exp(gate / 2), two
+    units in the last place (4 U) each, and three products: 11 U.  The scale adds its division, a value e4m3's half step and both."""
+    torch = torch_cuda
+    x = torch.empty((rows, 2 * columns), device="cuda")
+    x[:, :columns] = -88.75 - 14 * torch.rand((rows, columns), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    x[:, columns:] = 1e30 * randn(torch, 4, rows, columns)
+    x = x.to(getattr(torch, dtype))
+    values, scales = sampler.quantize_rows(x, activation=pkg.ACTIVATION_SILU_GATE)
+    gate, up = x.double()[:, :columns], x.double()[:, columns:]
+    h = gate * torch.sigmoid(gate) * up
+    padded = torch.nn.functional.pad(h, (0, -columns % 128)).view(rows, -1, 128)
+    want = (padded.abs().amax(dim=2) / 448).t()
+    assert bool((want > 1e-30).all()) and bool(((scales.double() - want).abs() <= 13 * U * want).all())
+    wide = scales.double().t().repeat_interleave(128, dim=1)[:, :columns]
+    off = (values.double() * wide - h).abs()
+    assert bool((off <= (2.0 ** -4 + 32 * U) * h.abs().clamp_min(2.0 ** -6 * wide)).all())
+
+
+def test_quantize_gate_of_infinities(sampler, pkg, torch_cuda):
+    """NaN where the formula has none, and only there: -inf / inf, and 0 times an infinity."""
+    torch = torch_cuda
+    inf = float("inf")
+    gate = torch.tensor([-inf, -300.0, -89.0, 0.0, 5.0, inf, 5.0, float("nan")], device="cuda")
+    up = torch.tensor([1.0, 1.0, 1.0, inf, 2.0, 0.0, 0.0, 1.0], device="cuda")
+    values, scales = sampler.quantize_rows(torch.cat([gate, up])[None], activation=pkg.ACTIVATION_SILU_GATE)
+    decoded = values.float()[0] * scales[0]
+    assert torch.isnan(decoded).tolist() == [True, False, False, True, False, True, False, True]
+    assert decoded[[1, 2, 6]].abs().max() == 0    # far below the block's largest, or zero
+    assert abs(float(decoded[4]) - 10 / (1 + 2.718281828459045 ** -5)) <= 2.0 ** -4 * 10
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "sqrtsoftplus"])
 @pytest.mark.parametrize("experts", [24, 256, 1000, 1500])
 @pytest.mark.parametrize("lowest", [float("-inf"), -3.4028234663852886e38])
