@@ -10,6 +10,7 @@ The directory name is not a Python identifier; load it with
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 from dataclasses import dataclass
@@ -229,8 +230,26 @@ def _rows_address(tensor, name, device):
     return tensor.data_ptr()
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _results_on(device, stream):
+    """Context in which a call on the stream handle `stream` makes its results.  Made on the current stream instead, their memory could
+    still be in use there, be filled there after the call's kernels have written it, or be handed out while they write."""
+    if stream is None:
+        return _HERE
+    import torch
+    if stream == torch.cuda.current_stream(device).cuda_stream:
+        return _HERE
+    return torch.cuda.stream(torch.cuda.default_stream(device) if stream == 0 else torch.cuda.ExternalStream(stream, device=device))
+
+
 class Sampler:
-    """One moe_sampler handle."""
+    """One moe_sampler handle.
+
+    Methods that take `stream` (a CUDA stream handle; the current stream unless given) make the results that they return on it: use
+    them there, or order the use behind it.  Inputs have to be ready on that stream and, where they were made on another one, to be
+    kept until it is done with them."""
 
     def __init__(self, max_rows: int, max_vocab: int, device: int = 0):
         self._lib = library()
@@ -274,13 +293,14 @@ class Sampler:
             raise TypeError("logits must be float32 or bfloat16")
         device = logits.device
         if out is None:
-            out = {
-                "token": torch.empty(rows, dtype=torch.int32, device=device),
-                "probability": torch.empty(rows, dtype=torch.float32, device=device),
-                "flags": torch.empty(rows, dtype=torch.int32, device=device),
-                "status": torch.empty(rows, dtype=torch.int32, device=device),
-                "topk": torch.empty((rows, topk_stride), dtype=torch.int32, device=device) if topk_stride else None,
-            }
+            with _results_on(device, stream):
+                out = {
+                    "token": torch.empty(rows, dtype=torch.int32, device=device),
+                    "probability": torch.empty(rows, dtype=torch.float32, device=device),
+                    "flags": torch.empty(rows, dtype=torch.int32, device=device),
+                    "status": torch.empty(rows, dtype=torch.int32, device=device),
+                    "topk": torch.empty((rows, topk_stride), dtype=torch.int32, device=device) if topk_stride else None,
+                }
         offsets = tokens = None
         if stop_lists is not None:
             offsets, tokens = stop_lists_to_csr(stop_lists)
@@ -290,9 +310,10 @@ class Sampler:
         stream_handle = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
         if kept_stride:
             if "kept_count" not in out:
-                out["kept_count"] = torch.empty(rows, dtype=torch.int32, device=device)
-                out["kept_token"] = torch.full((rows, kept_stride), -1, dtype=torch.int32, device=device)
-                out["kept_probability"] = torch.zeros((rows, kept_stride), dtype=torch.float32, device=device)
+                with _results_on(device, stream):
+                    out["kept_count"] = torch.empty(rows, dtype=torch.int32, device=device)
+                    out["kept_token"] = torch.full((rows, kept_stride), -1, dtype=torch.int32, device=device)
+                    out["kept_probability"] = torch.zeros((rows, kept_stride), dtype=torch.float32, device=device)
             outputs = SampleOutputs(_dev_ptr(out["token"]), _dev_ptr(out["probability"]), _dev_ptr(out["flags"]), _dev_ptr(out["status"]),
                                     _dev_ptr(out.get("topk")), int(topk_stride), _dev_ptr(out["kept_token"]), _dev_ptr(out["kept_probability"]),
                                     _dev_ptr(out["kept_count"]), int(kept_stride))
@@ -338,8 +359,9 @@ class Sampler:
         device = target_logits.device
         params = np.ascontiguousarray(params, dtype=ROW_PARAMS_DTYPE).reshape(1)
         if out is None:
-            out = (torch.zeros(max(draft_count, 1), dtype=torch.float32, device=device),
-                   torch.zeros(SPECULATIVE_RESULT_DTYPE.itemsize, dtype=torch.uint8, device=device))
+            with _results_on(device, stream):
+                out = (torch.zeros(max(draft_count, 1), dtype=torch.float32, device=device),
+                       torch.zeros(SPECULATIVE_RESULT_DTYPE.itemsize, dtype=torch.uint8, device=device))
         accepted_probability, result = out
         stream_handle = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_speculative_verify(self._handle, C.c_void_p(stream_handle), _dev_ptr(target_logits),
@@ -370,8 +392,9 @@ class Sampler:
         device = target_logits.device
         params = np.ascontiguousarray(params, dtype=ROW_PARAMS_DTYPE).reshape(sessions)
         if out is None:
-            out = (torch.zeros(max(sessions * draft_count, 1), dtype=torch.float32, device=device),
-                   torch.zeros(max(sessions, 1) * SPECULATIVE_RESULT_DTYPE.itemsize, dtype=torch.uint8, device=device))
+            with _results_on(device, stream):
+                out = (torch.zeros(max(sessions * draft_count, 1), dtype=torch.float32, device=device),
+                       torch.zeros(max(sessions, 1) * SPECULATIVE_RESULT_DTYPE.itemsize, dtype=torch.uint8, device=device))
         accepted_probability, result = out
         stream_handle = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_speculative_verify_batch(self._handle, C.c_void_p(stream_handle), _dev_ptr(target_logits),
@@ -441,7 +464,8 @@ class Sampler:
         import torch
         rows, row_stride = logits.shape
         dtype = DTYPE_F32 if logits.dtype == torch.float32 else DTYPE_BF16
-        candidates = torch.empty((rows, top_k), dtype=torch.int64, device=logits.device) if out is None else out
+        with _results_on(logits.device, stream):
+            candidates = torch.empty((rows, top_k), dtype=torch.int64, device=logits.device) if out is None else out
         stream_handle = torch.cuda.current_stream(logits.device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_sample_local_candidates(self._handle, C.c_void_p(stream_handle), _dev_ptr(logits), dtype, rows, row_stride,
                                                           logits.stride(0), int(vocab_begin), int(top_k), _dev_ptr(candidates)))
@@ -453,13 +477,14 @@ class Sampler:
         shards, rows, k = gathered.shape
         assert k == top_k
         device = gathered.device
-        out = out if out is not None else {
-            "token": torch.empty(rows, dtype=torch.int32, device=device),
-            "probability": torch.empty(rows, dtype=torch.float32, device=device),
-            "flags": torch.empty(rows, dtype=torch.int32, device=device),
-            "status": torch.empty(rows, dtype=torch.int32, device=device),
-            "topk": torch.empty((rows, topk_stride), dtype=torch.int32, device=device) if topk_stride else None,
-        }
+        with _results_on(device, stream):
+            out = out if out is not None else {
+                "token": torch.empty(rows, dtype=torch.int32, device=device),
+                "probability": torch.empty(rows, dtype=torch.float32, device=device),
+                "flags": torch.empty(rows, dtype=torch.int32, device=device),
+                "status": torch.empty(rows, dtype=torch.int32, device=device),
+                "topk": torch.empty((rows, topk_stride), dtype=torch.int32, device=device) if topk_stride else None,
+            }
         if params is not None:   # None reuses the parameters uploaded by the previous call
             params = np.ascontiguousarray(params, dtype=ROW_PARAMS_DTYPE)
         stream_handle = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
@@ -502,9 +527,10 @@ class Sampler:
                                 explicit_ids.data_ptr() if explicit_ids is not None else None)
         routes = token_count * top_k
         if out is None:
-            out = DispatchPlan(torch.empty(expert_count + 1, dtype=torch.int32, device=device), torch.empty(routes, dtype=torch.int32, device=device),
-                               torch.empty(routes, dtype=torch.int32, device=device), torch.empty(routes, dtype=torch.float32, device=device),
-                               torch.zeros(1, dtype=torch.int32, device=device))
+            with _results_on(device, stream):
+                out = DispatchPlan(torch.empty(expert_count + 1, dtype=torch.int32, device=device), torch.empty(routes, dtype=torch.int32, device=device),
+                                   torch.empty(routes, dtype=torch.int32, device=device), torch.empty(routes, dtype=torch.float32, device=device),
+                                   torch.zeros(1, dtype=torch.int32, device=device))
         stream_handle = torch.cuda.current_stream(device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_router_dispatch(self._handle, C.c_void_p(stream_handle), _dev_ptr(router_logits), token_count, C.byref(options),
                                                   _dev_ptr(out.expert_offsets), _dev_ptr(out.route_token), _dev_ptr(out.route_rank),
@@ -515,7 +541,8 @@ class Sampler:
         import torch
         token_count, columns = hidden.shape
         routes = route_token.numel()
-        gathered = torch.empty((routes, columns), dtype=torch.float32, device=hidden.device)
+        with _results_on(hidden.device, stream):
+            gathered = torch.empty((routes, columns), dtype=torch.float32, device=hidden.device)
         stream_handle = torch.cuda.current_stream(hidden.device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_regroup_gather(self._handle, C.c_void_p(stream_handle), _dev_ptr(hidden), token_count, columns,
                                                  _dev_ptr(route_token), routes, _dev_ptr(gathered)))
@@ -527,8 +554,9 @@ class Sampler:
         import torch
         rows, row_stride = scores.shape
         count = row_stride if count is None else count
-        indices = torch.empty((rows, top_k), dtype=torch.int32, device=scores.device)
-        values = torch.empty((rows, top_k), dtype=torch.float32, device=scores.device) if with_scores else None
+        with _results_on(scores.device, stream):
+            indices = torch.empty((rows, top_k), dtype=torch.int32, device=scores.device)
+            values = torch.empty((rows, top_k), dtype=torch.float32, device=scores.device) if with_scores else None
         stream_handle = torch.cuda.current_stream(scores.device).cuda_stream if stream is None else stream
         self._check(self._lib.moe_indexer_topk(self._handle, C.c_void_p(stream_handle), _dev_ptr(scores), rows, int(count), scores.stride(0), int(top_k),
                                                _dev_ptr(indices), _dev_ptr(values)))
@@ -568,8 +596,9 @@ class Sampler:
         rows = source_rows if route_token is None else route_token.numel()
         blocks = (columns + EXPERT_BLOCK - 1) // EXPERT_BLOCK
         if out is None:
-            values = torch.empty(rows, columns, dtype=torch.float8_e4m3fn, device=source.device)
-            scales = torch.empty(blocks, rows, dtype=torch.float32, device=source.device)
+            with _results_on(device, stream):
+                values = torch.empty(rows, columns, dtype=torch.float8_e4m3fn, device=source.device)
+                scales = torch.empty(blocks, rows, dtype=torch.float32, device=source.device)
             values_address, scales_address = values.data_ptr(), scales.data_ptr()
         else:
             values, scales = out
@@ -593,7 +622,8 @@ class Sampler:
         experts, outputs, _ = weights.shape
         blocks = (columns + EXPERT_BLOCK - 1) // EXPERT_BLOCK
         if out is None:
-            out = torch.empty(rows, outputs, dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=values.device)
+            with _results_on(device, stream):
+                out = torch.empty(rows, outputs, dtype=torch.bfloat16 if out_dtype is None else out_dtype, device=values.device)
         elif out.shape != (rows, outputs):
             raise ValueError(f"out must have shape {(rows, outputs)}, got {tuple(out.shape)}")
         self._check(self._lib.moe_expert_product(
@@ -614,7 +644,8 @@ class Sampler:
         address = _rows_address(route_rows, "route_rows", device)
         routes, columns = route_rows.shape
         if out is None:
-            out = torch.empty(token_count, columns, dtype=route_rows.dtype, device=route_rows.device)
+            with _results_on(device, stream):
+                out = torch.empty(token_count, columns, dtype=route_rows.dtype, device=route_rows.device)
             out_address = out.data_ptr()
         else:
             out_address = _address(out, "out", (token_count, columns), route_rows.dtype, device)
@@ -640,8 +671,9 @@ class Sampler:
         tokens, experts = router_logits.shape
         if out is None:
             place = router_logits.device
-            out = BalanceLoss(torch.empty(1, dtype=torch.float32, device=place), torch.empty(experts + 1, dtype=torch.int32, device=place),
-                              torch.empty(experts, dtype=torch.float32, device=place))
+            with _results_on(device, stream):
+                out = BalanceLoss(torch.empty(1, dtype=torch.float32, device=place), torch.empty(experts + 1, dtype=torch.int32, device=place),
+                                  torch.empty(experts, dtype=torch.float32, device=place))
             results = out.expert_tokens.data_ptr(), out.expert_probability.data_ptr(), out.loss.data_ptr()
         else:
             results = (_address(out.expert_tokens, "expert_tokens", (experts + 1,), torch.int32, device),
@@ -667,7 +699,8 @@ class Sampler:
         device = self.device
         tokens, experts = router_logits.shape
         if out is None:
-            out = torch.empty(tokens, experts, dtype=torch.float32, device=router_logits.device)
+            with _results_on(device, stream):
+                out = torch.empty(tokens, experts, dtype=torch.float32, device=router_logits.device)
             out_address = out.data_ptr()
         else:
             out_address = _address(out, "out", (tokens, experts), torch.float32, device)
