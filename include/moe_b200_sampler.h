@@ -317,7 +317,9 @@ typedef struct moe_router_options
  *     experts ascending, inside an expert token ascending then rank ascending
  *   plan_status[1]  0, or a router status value (see moe_router_status_message)
  * Asynchronous on `stream`; the shape checks that need no data are done on the
- * host and returned directly. */
+ * host and returned directly.  The first call on a handle, and one with more routes
+ * or experts than any before, allocates scratch: make it before a stream capture,
+ * where it is refused.  Graphs captured earlier stay valid. */
 int moe_router_dispatch(moe_sampler* sampler, void* stream, const float* router_logits, uint32_t token_count,
                         const moe_router_options* options, uint32_t* expert_offsets, uint32_t* route_token,
                         uint32_t* route_rank, float* route_weight, int32_t* plan_status);

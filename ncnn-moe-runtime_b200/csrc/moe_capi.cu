@@ -931,25 +931,17 @@ int moe_router_dispatch(moe_sampler* sampler, void* stream_handle, const float* 
     cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
     DeviceGuard guard(sampler->device);
     const size_t routes = static_cast<size_t>(token_count) * options->top_k;
-    if (routes > sampler->selected_capacity || options->expert_count > sampler->expert_counts_capacity || sampler->router_block_counts == nullptr)
-    {
-        // earlier calls on this stream may still use the scratch that is replaced here
-        MOE_CUDA_CHECK(sampler, cudaStreamSynchronize(stream));
-        if (routes > sampler->selected_capacity)
-        {
-            size_t capacity = sampler->selected_capacity;
-            MOE_CUDA_CHECK(sampler, grow(sampler->selected_expert, capacity, routes));
-            MOE_CUDA_CHECK(sampler, grow(sampler->selected_weight, sampler->selected_capacity, routes));
-        }
-        // every call rewrites the counts it reads (per block, then per expert): nothing to clear
-        if (options->expert_count > sampler->expert_counts_capacity)
-            MOE_CUDA_CHECK(sampler, grow(sampler->expert_counts, sampler->expert_counts_capacity, options->expert_count));
-        if (sampler->router_block_counts == nullptr)
-        {
-            size_t capacity = 0;
-            MOE_CUDA_CHECK(sampler, grow(sampler->router_block_counts, capacity, MOE_ROUTER_BLOCK_TABLE_ENTRIES));
-        }
-    }
+    // every call rewrites what it reads there (routes; counts per block, then per expert): nothing to clear
+    size_t capacity = sampler->selected_capacity;
+    if (int status = grow_scratch(sampler, sampler->selected_expert, capacity, routes, stream, false))
+        return status;
+    if (int status = grow_scratch(sampler, sampler->selected_weight, sampler->selected_capacity, routes, stream, false))
+        return status;
+    if (int status = grow_scratch(sampler, sampler->expert_counts, sampler->expert_counts_capacity, options->expert_count, stream, false))
+        return status;
+    capacity = sampler->router_block_counts != nullptr ? MOE_ROUTER_BLOCK_TABLE_ENTRIES : 0u;
+    if (int status = grow_scratch(sampler, sampler->router_block_counts, capacity, MOE_ROUTER_BLOCK_TABLE_ENTRIES, stream, false))
+        return status;
     RouterArgs args = {};
     args.logits = router_logits;
     args.token_count = token_count;

@@ -71,6 +71,41 @@ def test_balance_refuses_to_grow_inside_a_capture(pkg, torch_cuda):
         handle.close()
 
 
+def test_a_captured_dispatch_outlives_larger_ones(pkg, torch_cuda):
+    """The scratch that a graph was captured with stays when a later call needs more."""
+    torch = torch_cuda
+    handle = pkg.Sampler(max_rows=1, max_vocab=64)
+
+    def fields(plan):
+        return [t.clone() for t in (plan.expert_offsets, plan.route_token, plan.route_rank, plan.route_weight, plan.status)]
+
+    try:
+        small, large = randn(torch, 1, 300, 16), randn(torch, 2, 40000, 200)
+        side = torch.cuda.Stream()
+        want, plan = handle.router_dispatch(small, 2), handle.router_dispatch(small, 2)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            handle.router_dispatch(small, 2, out=plan)
+            with pytest.raises(pkg.MoeError, match="inside a stream capture"):
+                handle.router_dispatch(large, 4)
+        first = None
+        for _ in range(3):
+            for t in (plan.expert_offsets, plan.route_token, plan.route_rank, plan.route_weight):
+                t.zero_()
+            plan.status.fill_(-1)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                other = handle.router_dispatch(large, 4)
+                graph.replay()
+            side.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(fields(plan), fields(want)))
+            assert first is None or all(torch.equal(a, b) for a, b in zip(fields(other), first))
+            first = fields(other)
+    finally:
+        handle.close()
+
+
 def often_routed(torch, source_rows, columns):
     """Rows that are quantised once and copied: 4.5 routes a row, 2^25 values and more."""
     routes = source_rows * 9 // 2
