@@ -894,14 +894,14 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
 
 EncodeTiled encode_function()
 {
-    static const EncodeTiled function = [] {
+    static std::atomic<EncodeTiled> found{nullptr};
+    return found_once(found, [] {
         void* entry = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &result) != cudaSuccess || result != cudaDriverEntryPointSuccess)
             entry = nullptr;
         return reinterpret_cast<EncodeTiled>(entry);
-    }();
-    return function;
+    });
 }
 
 // Rows of `columns` bytes, read in boxes of `box_rows` rows by 128 columns; zeros behind the last column and row.

@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <mutex>
 #include <new>
 #include <string>
@@ -270,6 +271,20 @@ ClusterOccupancy cluster_occupancy(ClusterOccupancyTable& table, int device, Que
         table.known[device] = true;
     }
     return found;
+}
+
+// A function that is looked up at run time: remembered once it is found.  A look-up that fails serves one call alone.
+template<typename Function, typename LookUp>
+Function found_once(std::atomic<Function>& found, LookUp look_up)
+{
+    Function function = found.load(std::memory_order_acquire);
+    if (function == nullptr)
+    {
+        function = look_up();
+        if (function != nullptr)
+            found.store(function, std::memory_order_release);
+    }
+    return function;
 }
 
 // Scratch of calls that may be captured: what a captured graph was given stays allocated (in `kept`) until the handle goes, so
