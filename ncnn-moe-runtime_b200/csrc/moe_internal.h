@@ -456,6 +456,12 @@ inline size_t quantize_once_bytes(const QuantizeArgs& a)
 bool combine_few(uint32_t route_count, uint32_t token_count, uint32_t top_k);
 cudaError_t launch_expert_product(const ProductArgs& args, int out_dtype, int sm_count, cudaStream_t stream);
 cudaError_t launch_combine_routes(const CombineArgs& args, int dtype, cudaStream_t stream);
+// Blocks of `warps` tokens each at a time, `most` of them at most.
+inline uint32_t balance_blocks(uint32_t token_count, uint32_t warps, uint32_t most)
+{
+    const uint32_t wanted = token_count / warps + (token_count % warps != 0u ? 1u : 0u);
+    return wanted < most ? wanted : most;
+}
 cudaError_t launch_balance_loss(const BalanceArgs& args, cudaStream_t stream);
 cudaError_t launch_balance_loss_backward(const BalanceArgs& args, const uint32_t* expert_tokens, const float* loss_gradient, float* gradient, cudaStream_t stream);
 
