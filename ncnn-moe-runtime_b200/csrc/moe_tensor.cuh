@@ -8,7 +8,7 @@
 
 namespace moe {
 
-constexpr uint32_t kSpinLimit = 1u << 20; // looks at a barrier before a wait gives up
+constexpr uint32_t kSpinLimit = 1u << 20; // looks at a barrier before a wait gives up: one that fails is held for 4 us, so 4 s
 
 // ---- mbarriers, tensor memory, descriptors ---------------------------------------------
 
@@ -55,12 +55,12 @@ __device__ __forceinline__ bool barrier_test(uint32_t barrier, uint32_t parity)
 }
 // Bounded.  A wait that runs out marks the CTA as stalled; every role then leaves its loop.  The first look is apart from the
 // loop: most waits find their phase complete, and a look costs 16 cycles where the loop takes 85.
-__device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, volatile uint32_t* stalled)
+__device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, volatile uint32_t* stalled, uint32_t limit = kSpinLimit)
 {
     if (barrier_test(barrier, parity))
         return true;
 #pragma unroll 1
-    for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
+    for (uint32_t spin = 0; spin < limit; ++spin)
     {
         if (barrier_test(barrier, parity))
             return true;
@@ -71,12 +71,12 @@ __device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, 
     return false;
 }
 // The same for a whole warp, which stays together.
-__device__ __forceinline__ bool barrier_wait_warp(uint32_t barrier, uint32_t parity, volatile uint32_t* stalled)
+__device__ __forceinline__ bool barrier_wait_warp(uint32_t barrier, uint32_t parity, volatile uint32_t* stalled, uint32_t limit = kSpinLimit)
 {
     if (__all_sync(kFullMask, barrier_test(barrier, parity)))
         return true;
 #pragma unroll 1
-    for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
+    for (uint32_t spin = 0; spin < limit; ++spin)
     {
         if (__all_sync(kFullMask, barrier_test(barrier, parity)))
             return true;

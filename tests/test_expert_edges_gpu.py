@@ -1,7 +1,13 @@
-"""Edges of the expert calls on the GPU: scratch and stream captures.  Helpers and the rule for tolerances: tests/test_expert_gpu.py."""
+"""Edges of the expert calls on the GPU: scratch and stream captures, extreme values, waits that run out, offsets beyond 32 bits.
+Helpers and the rule for tolerances: tests/test_expert_gpu.py."""
+import ctypes
+import shutil
+import subprocess
+from pathlib import Path
+
 import pytest
 
-from test_expert_gpu import U, combine_reference, plan_of, randn, score_code
+from test_expert_gpu import U, assert_product, blocks_of, combine_reference, plan_of, product_reference, randn, score_code
 
 pytestmark = pytest.mark.gpu
 
@@ -209,3 +215,77 @@ def test_balance_of_tokens_masked_for_every_expert(sampler, pkg, torch_cuda, sco
     gradient = sampler.balance_loss_backward(logits, out.expert_tokens, 3, score_function=code)
     assert bool((gradient[4] == 0).all()) and bool(torch.isfinite(gradient).all())
     assert bool((gradient[9, 1:] == 0).all())
+
+
+def test_waits_run_out(torch_cuda):
+    """tests/cuda/waits.cu: a wait for what never comes ends, marks the CTA, and ends the waits of the other warps."""
+    source = Path(__file__).resolve().parent / "cuda" / "waits.cu"
+    target = source.with_name("libtest_waits.so")
+    csrc = source.parent.parent.parent / "ncnn-moe-runtime_b200" / "csrc"
+    inputs = [source, csrc / "moe_tensor.cuh", csrc / "moe_common.cuh"]
+    if not target.exists() or any(path.stat().st_mtime > target.stat().st_mtime for path in inputs):
+        nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+        subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-o", str(target), str(source)], check=True)
+    results, microseconds = (ctypes.c_int * 7)(), ctypes.c_float()
+    library = ctypes.CDLL(str(target))
+    assert library.test_waits(ctypes.c_uint32(1000), results, ctypes.byref(microseconds)) == 0
+    assert list(results) == [0, 1, 0, 0, 1, 1, 1]
+    assert microseconds.value < 1e6     # two times 1000 looks of 4 us, and the 64000 looks cut short
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("source_rows,routes,columns", [(50, 173, 40), (50, 173, 264), (300, 1100, 4096), (1000, 33000, 1040), (1000, 33000, 1032)])
+def test_quantize_gates_routed_rows(sampler, pkg, torch_cuda, dtype, source_rows, routes, columns):
+    """Gate and route in one call, route by route and with rows quantised once: the bits of the gated rows, gathered."""
+    torch = torch_cuda
+    source = (2 * randn(torch, 7, source_rows, 2 * columns)).to(getattr(torch, dtype))
+    index = torch.randint(source_rows, (routes,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").int()
+    rows, row_scales = sampler.quantize_rows(source, activation=pkg.ACTIVATION_SILU_GATE)
+    values, scales = sampler.quantize_rows(source, route_token=index, activation=pkg.ACTIVATION_SILU_GATE)
+    want, want_scales = rows.view(torch.uint8)[index.long()], row_scales[:, index.long()]
+    assert torch.equal(values.view(torch.uint8), want) and torch.equal(scales, want_scales)
+    assert sampler.expert_check() == 0
+    index[[5, routes - 1]] = torch.tensor([source_rows, -1], dtype=torch.int32, device="cuda")
+    values, scales = sampler.quantize_rows(source, route_token=index, activation=pkg.ACTIVATION_SILU_GATE)
+    assert sampler.expert_check() == pkg.EXPERT_FLAG_TOKEN_RANGE
+    want[[5, routes - 1]] = 0
+    want_scales[:, [5, routes - 1]] = 0
+    assert torch.equal(values.view(torch.uint8), want) and torch.equal(scales, want_scales)
+
+
+# experts, rows of all, outputs, columns: which kernel, and what has more than 2^32 bytes or values
+BEYOND = [pytest.param(70, 70 * 20, 8192, 8208, id="tiles of 32 rows, weights"), pytest.param(70, 70 * 33, 128, 480000, id="tiles of 64 rows, weights"),
+          pytest.param(70, 70 * 40, 8192, 8208, id="many rows, weights"), pytest.param(4096, 65536, 16, 65552, id="tiles of 16 rows, values and weights"),
+          pytest.param(1, 530000, 16, 8208, id="many rows, values"), pytest.param(4096, 65536, 65600, 16, id="tiles of 16 rows, outputs"),
+          pytest.param(1, (1 << 22) + 200, 1040, 16, id="many rows, outputs in whole lines"), pytest.param(1, (1 << 22) + 200, 1039, 16, id="many rows, outputs anywhere")]
+
+
+@pytest.mark.parametrize("experts,rows,outputs,columns", BEYOND)
+def test_products_beyond_32_bits(sampler, torch_cuda, experts, rows, outputs, columns):
+    """The last rows, of the last expert; all others are zeros."""
+    torch = torch_cuda
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    last = 16 if experts == 4096 else 40
+    values = torch.zeros((rows, columns), dtype=torch.float8_e4m3fn, device="cuda")
+    values[-last:] = (randn(torch, 3, last, columns) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    weights = torch.zeros((experts, outputs, columns), dtype=torch.float8_e4m3fn, device="cuda")
+    weights[-1] = (randn(torch, 2, outputs, columns) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = torch.ones((blocks_of(columns), rows), device="cuda")
+    weight_scales = torch.ones((experts, blocks_of(outputs), blocks_of(columns)), device="cuda")
+    scales[:, -last:] = torch.rand((blocks_of(columns), last), generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") + 0.1
+    if experts == 4096:
+        offsets = 16 * torch.arange(experts + 1, dtype=torch.int32, device="cuda")
+    else:   # the first expert and the last one
+        offsets = torch.full((experts + 1,), rows - last, dtype=torch.int32, device="cuda")
+        offsets[0], offsets[-1] = 0, rows
+    out = torch.full((rows, outputs), -7.0, dtype=torch.bfloat16, device="cuda")
+    sampler.expert_product(values, scales, weights, weight_scales, expert_offsets=offsets if experts > 1 else None, out=out)
+    one = torch.tensor([0, last], dtype=torch.int32, device="cuda")
+    reference = product_reference(torch, values[-last:], scales[:, -last:].contiguous(), weights[-1:], weight_scales[-1:], one)
+    assert_product(torch, out[-last:], reference, columns)
+    for first in range(0, rows - last, 1 << 18):
+        assert not bool(out[first:min(first + (1 << 18), rows - last)].any())
+    assert sampler.expert_check() == 0
+    del values, weights, out, reference
+    torch.cuda.empty_cache()
