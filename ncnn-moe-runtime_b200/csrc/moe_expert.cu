@@ -77,7 +77,6 @@ struct Eight
 // reduced side by side until a lane has one of them, and it divides and inverts that one.
 
 constexpr int kQuantizeThreads = 128;
-constexpr uint32_t kQuantizeItem = 256u; // columns of an item, by its steps: the blocks of 128 that a half warp takes from it
 constexpr float kE4m3Max = 448.0f;
 
 __device__ __forceinline__ uint32_t to_e4m3_pair(float low, float high)
@@ -156,13 +155,13 @@ __global__ void __launch_bounds__(kQuantizeThreads, kQuantizeBlocks<T, kGate, kS
     wait_for_previous_kernel();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t half = lane >> 4, sub = lane & 15u;
-    const uint32_t pieces = (a.columns + kQuantizeItem * kSteps - 1u) / (kQuantizeItem * kSteps);
+    const uint32_t pieces = (a.columns + MOE_QUANTIZE_ITEM * kSteps - 1u) / (MOE_QUANTIZE_ITEM * kSteps);
     const uint64_t items = static_cast<uint64_t>(a.rows) * pieces;
     const uint64_t stride = static_cast<uint64_t>(gridDim.x) * (kQuantizeThreads / 32);
     for (uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kQuantizeThreads / 32) + (threadIdx.x >> 5); item < items; item += stride)
     {
         const uint32_t row = static_cast<uint32_t>(item / pieces);
-        const uint32_t first = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * pieces) * (kQuantizeItem * kSteps);
+        const uint32_t first = static_cast<uint32_t>(item - static_cast<uint64_t>(row) * pieces) * (MOE_QUANTIZE_ITEM * kSteps);
         uint32_t source_row = row;
         bool valid = true;
         if (a.route_token != nullptr)
@@ -323,24 +322,18 @@ __global__ void __launch_bounds__(kSpreadThreads) spread_rows_kernel(const Quant
 template<typename T, int kSteps>
 cudaError_t launch_quantize_steps(const QuantizeArgs& a, bool gate, cudaStream_t stream)
 {
-    const uintptr_t bases = reinterpret_cast<uintptr_t>(a.source);
-    const bool vector = a.columns % 8u == 0u && bases % 16u == 0u && a.row_stride * sizeof(T) % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 8u == 0u;
-    const uint64_t items = static_cast<uint64_t>(a.rows) * ((a.columns + kQuantizeItem * kSteps - 1u) / (kQuantizeItem * kSteps));
+    const bool vector = quantize_in_vectors(a, sizeof(T));
+    const uint64_t items = static_cast<uint64_t>(a.rows) * ((a.columns + MOE_QUANTIZE_ITEM * kSteps - 1u) / (MOE_QUANTIZE_ITEM * kSteps));
     const uint64_t blocks = (items + kQuantizeThreads / 32 - 1) / (kQuantizeThreads / 32);
     const uint32_t grid = static_cast<uint32_t>(blocks < 148u * 16u ? blocks : 148u * 16u);
     auto kernel = gate ? (vector ? quantize_rows_kernel<T, true, true, kSteps> : quantize_rows_kernel<T, true, false, kSteps>)
                        : (vector ? quantize_rows_kernel<T, false, true, kSteps> : quantize_rows_kernel<T, false, false, kSteps>);
     return launch_following(kernel, grid, kQuantizeThreads, 0, stream, a);
 }
-// Small calls wait for one item's latency, so they are cut finer: 128 x 2880 fp32 gated 2.6 us with one step, 4.1 with four; 256 x
-// 4096 bf16 2.3 against 2.8, 1024 x 4096 gated 7.2 against 7.7.  Above, the divisions that four blocks share pay: 512 x 4096 3.3
-// against 3.5, 2048 x 4096 gated 12.5 against 13.9, 4096 x 4096 11.3 against 15.4.
 template<typename T>
 cudaError_t launch_quantize(const QuantizeArgs& a, bool gate, cudaStream_t stream)
 {
-    if (static_cast<uint64_t>(a.rows) * a.columns <= (gate ? 1ull << 22 : 1ull << 20))
-        return launch_quantize_steps<T, 1>(a, gate, stream);
-    return launch_quantize_steps<T, 4>(a, gate, stream);
+    return quantize_steps(a, sizeof(T), gate) == 4u ? launch_quantize_steps<T, 4>(a, gate, stream) : launch_quantize_steps<T, 1>(a, gate, stream);
 }
 
 // ---- combine --------------------------------------------------------------------------

@@ -20,6 +20,8 @@
 #define MOE_SPECULATIVE_SHORT_LIST 1024u
 // entries of the router's [expert][block] count table (expert_count * blocks of the select kernel never exceeds it)
 #define MOE_ROUTER_BLOCK_TABLE_ENTRIES 262144u
+// columns of an item of the quantisation, by its steps: the blocks of 128 that a half warp takes from it
+#define MOE_QUANTIZE_ITEM 256u
 // blocks of the balance loss's first kernel (its scratch holds one partial sum per block and expert): two per SM
 #define MOE_BALANCE_MAX_BLOCKS 296u
 
@@ -451,6 +453,29 @@ inline size_t quantize_once_bytes(const QuantizeArgs& a)
     const bool worth = a.route_token != nullptr && a.rows / 4u >= a.source_rows && static_cast<uint64_t>(a.rows) * a.columns >= (1ull << 25);
     const bool fits = a.columns % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 16u == 0u && a.source_rows > 0u && bytes <= kQuantizeOnceBytes;
     return worth && fits ? bytes : 0u;
+}
+// whether rows of source and values can be moved in vectors of eight values
+inline bool quantize_in_vectors(const QuantizeArgs& a, size_t element)
+{
+    return a.columns % 8u == 0u && reinterpret_cast<uintptr_t>(a.source) % 16u == 0u && a.row_stride * element % 16u == 0u && reinterpret_cast<uintptr_t>(a.values) % 8u == 0u;
+}
+// Steps of a warp's item: four blocks a half warp share their divisions, in one pass over 1024 columns of a row, of which lanes stay
+// empty where the row ends inside them; small calls wait for one item's latency.  So four steps are for calls of many values whose
+// pieces of 256 columns fill those of 1024, to a share that hangs on what a value costs beside the divisions.  us with one and four
+// steps, inputs from memory:
+//   bf16        768 x 4096 4.1, 4.9; 1024 x 4096 5.5, 5.1; 2^25 values: x 256 31, 107; x 768 31, 40; x 1792 31, 32; x 2880 36, 28; x 5760 33, 29; x 4096 31, 24
+//   bf16 gated  1024 x 4096 8.0, 8.3; 1300 x 4096 10.7, 10.0; 2^25: x 256 56, 164; x 768 56, 58; x 1280 57, 68; x 1792 57, 50; x 4096 57, 44
+//   fp32        768 x 4096 4.4, 4.4; 1024 x 4096 5.4, 5.2; 2^25: x 256 28, 61; x 512 28, 34; x 1032 36, 33; x 2056 33, 29; x 4096 28, 27
+//   fp32 gated  1536 x 4096 12.4, 14.1; 2048 x 4096 16.5, 17.1; 2^25: x 256 59, 217; x 2056 66, 83; x 2880 63, 62; x 4096 59, 58
+//   rows that are not read in vectors: 1536 x 4095 bf16 11.8, 16.2, gated 15, 21; fp32 11.6, 13, gated 19, 20; 8194 x 4095 55, 54, 70, 74, 56, 54, 97, 89
+inline uint32_t quantize_steps(const QuantizeArgs& a, size_t element, bool gate)
+{
+    const bool wide = element == 4u;
+    const uint64_t most_small = gate && wide ? 16u << 20 : gate ? 4u << 20 : 3u << 20;                 // values
+    const uint64_t filled = gate ? (wide ? 24u : 20u) : (wide ? 15u : 22u);                            // pieces of 256 for six of 1024
+    const uint64_t pieces = (static_cast<uint64_t>(a.columns) + MOE_QUANTIZE_ITEM - 1u) / MOE_QUANTIZE_ITEM;
+    const bool many = static_cast<uint64_t>(a.rows) * a.columns > (quantize_in_vectors(a, element) ? most_small : 16u << 20);
+    return many && pieces * 6u >= (pieces + 3u) / 4u * filled ? 4u : 1u;
 }
 // whether a combine needs no slots: each of its CTAs looks through the routes
 bool combine_few(uint32_t route_count, uint32_t token_count, uint32_t top_k);

@@ -1,4 +1,4 @@
-"""CPU tests of what the expert calls do at their edges: scratch and stream captures, look-ups that fail, grids."""
+"""CPU tests of what the expert calls do at their edges: scratch and stream captures, look-ups that fail, grids and items."""
 from test_abi_cpu import run_host_test
 
 
@@ -15,3 +15,8 @@ def test_a_failed_look_up_is_made_again(tmp_path):
 def test_balance_grids_cover_the_largest_batches(tmp_path):
     """tests/cpp/balance_blocks_test.cpp: tokens of up to 2^32 - 1."""
     run_host_test(tmp_path, "balance_blocks_test")
+
+
+def test_quantisation_items_fit_the_rows(tmp_path):
+    """tests/cpp/quantize_steps_test.cpp: short rows and small calls are cut finer."""
+    run_host_test(tmp_path, "quantize_steps_test")

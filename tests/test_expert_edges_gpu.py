@@ -7,6 +7,7 @@ from pathlib import Path
 
 import pytest
 
+import test_expert_gpu
 from test_expert_gpu import U, assert_product, blocks_of, combine_reference, plan_of, product_reference, randn, score_code
 
 pytestmark = pytest.mark.gpu
@@ -159,7 +160,15 @@ def test_quantize_captured_before_any_scratch(pkg, torch_cuda):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("rows,columns", [(64, 300), (5000, 1032)])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,columns", [(1300, 4096), (4200, 4096), (4200, 4087), (9000, 2000), (30000, 640)])
+def test_quantize_wide_and_narrow_items(sampler, pkg, torch_cuda, dtype, gated, rows, columns):
+    """Calls that take the wide items, by type, gate and alignment, and long calls of short rows, which do not."""
+    test_expert_gpu.test_quantize_large_calls_are_their_parts(sampler, pkg, torch_cuda, dtype, gated, rows, columns)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,columns", [(64, 300), (1500, 4096)])
 def test_quantize_gate_far_below_zero(sampler, pkg, torch_cuda, dtype, rows, columns):
     """Gates whose exp(-gate) is beyond fp32 and ups that bring the product back: h = gate * e * up * e with e = exp(gate / 2), two
     units in the last place (4 U) each, and three products: 11 U.  The scale adds its division, a value e4m3's half step and both."""
