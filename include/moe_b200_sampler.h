@@ -7,7 +7,9 @@
  *
  * Threading: a handle serialises nothing.  Use one handle per host thread /
  * CUDA stream; calls on one handle must be issued in stream order on a single
- * stream because they share the handle's device workspace.
+ * stream because they share the handle's device workspace.  A graph captured from
+ * calls on a handle uses that workspace too: replay it in order with the handle's
+ * other calls and graphs, and before the handle is destroyed.
  *
  * There is no CPU fallback: every function that computes requires a CUDA
  * device of compute capability 10.x and fails with MOE_STATUS_CUDA_ERROR
@@ -424,7 +426,8 @@ int moe_quantize_rows(moe_sampler* sampler, void* stream, const void* source, in
 
 /* Each expert's rows times its weights, transposed:
  *   out[r, n] = sum over blocks b of scales[b, r] * weight_scales[e, n / 128, b] * sum over k in b of values[r, k] * weights[e, n, k]
- * e being the expert whose range [expert_offsets[e], expert_offsets[e + 1]) holds r.  Sums are fp32.
+ * e being the expert whose range [expert_offsets[e], expert_offsets[e + 1]) holds r.  Sums are fp32; the two scales of a block
+ * are multiplied first, in fp32, so their product should be a normal number.
  *
  * values, scales   device, as moe_quantize_rows writes them: [rows x columns], [ceil(columns / 128) x rows]
  * weights          device, [expert_count x outputs x columns] e4m3, dense

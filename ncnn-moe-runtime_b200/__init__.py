@@ -665,7 +665,8 @@ class Sampler:
     # ---- expert balance ----------------------------------------------------------------
     def balance_loss(self, router_logits, expert_offsets, route_token, top_k, score_function=ROUTER_SOFTMAX, token_mask=None, coefficient=1.0, stream=None,
                      out=None) -> BalanceLoss:
-        """moe_balance_loss: CUDA float32 logits [tokens, experts] and the plan made from them; token_mask bool / uint8 [tokens]."""
+        """moe_balance_loss: CUDA float32 logits [tokens, experts] and the plan made from them; token_mask bool / uint8 [tokens].
+        Nothing is recorded for autograd: the gradient with respect to the logits is balance_loss_backward's."""
         import torch
         device = self.device
         tokens, experts = router_logits.shape

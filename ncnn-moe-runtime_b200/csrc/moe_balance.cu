@@ -20,7 +20,7 @@ namespace moe {
 namespace {
 
 constexpr uint32_t kRegisterExperts = 1024; // up to here a lane holds a row's scores in registers
-// Threads of a block by the scores a lane holds; rows in shared memory (kPer 0) need 32 bytes a warp and expert.
+// Threads of a block by the scores a lane holds; rows in shared memory (kPer 0) need 8 bytes a warp and expert.
 template<int kPer>
 constexpr int kThreadsFor = kPer == 0 ? 128 : 512;
 // One wave of blocks: with twice as many, the second half waits for registers (32768 x 512, loss 22.9 against 25.6 us, gradient

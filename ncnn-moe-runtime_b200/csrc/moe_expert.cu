@@ -71,9 +71,9 @@ struct Eight
 // ---- quantisation -------------------------------------------------------------------
 //
 // scale = max |x| / 448 over a block of 128 columns, value = e4m3(x / scale).  Sixteen lanes own a block, eight values each, so
-// that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row (small calls: 256) and has all their loads in
+// that a bf16 row is read in 16-byte vectors; a warp takes 1024 columns of a row (or 256: quantize_steps) and has all their loads in
 // flight before the first maximum.  Large calls are bound by instructions before memory (16384 gated bf16 rows x 4096: 82 us,
-// 4.1 TB/s), so what belongs to a block is done once for the four blocks of a half warp: their maxima are
+// 4.1 TB/s, 72 % of the issue slots), so what belongs to a block is done once for the four blocks of a half warp: their maxima are
 // reduced side by side until a lane has one of them, and it divides and inverts that one.
 
 constexpr int kQuantizeThreads = 128;

@@ -3,11 +3,12 @@
 //
 // Per block of 128 columns the tensor cores compute the inner sums of a tile into a fresh accumulator in tensor memory, four
 // instructions of 32 columns each; other warps read it out and add it to their registers times the product of the two scales,
-// one fused multiply-add per element of the tile and block.  Two kernels:
+// itself rounded to fp32, one fused multiply-add per element of the tile and block.  Two kernels:
 //   few rows an expert   a tile is 128 outputs (the 128 lanes of an accumulator) by 16, 32 or 64 rows (its columns): the rows of
 //                        a decode step do not fill a tile of 128 with padding.  Bound by the weights from HBM.
 //   many rows            a tile is 128 rows by 256 outputs: a thread sums for one row, so that a block's factor is one register.
-//                        Bound by the sums or by the weights.
+//                        Bound by the weights, or by what eight warps can take out of tensor memory and sum: with 128 sums a thread no
+//                        others fit beside them to cover the waits (4096^3: tensor pipe 50 %, issue slots 49 %).
 // Roles of a CTA, which stays for all its tiles: a thread that requests tiles of both operands from the copy engine, threads
 // that issue the products, warps that scale, sum and store.  They pass a ring of operand stages and a few accumulators to each
 // other through mbarriers, so that copies, products and sums of different blocks, and of different tiles, overlap.
@@ -975,7 +976,8 @@ cudaError_t launch_many(const ProductArgs& a, int sm_count, cudaStream_t stream)
 // Experts are taken to have equal numbers of rows.  Up to 32 a tile of as many rows wastes least (64 experts of 32 rows x
 // 4096 x 4096: 32-row tiles 172 us, 64-row tiles 204, 128 x 256 tiles 187).  Above that the tiles' rates decide: a block of 64
 // rows by 128 outputs takes three fifths of the time of one of 128 by 256, so the smaller ones win while they are one wave (one
-// expert of 256 rows: 15.5 against 21.8 us) and lose from two on (512 rows: 27.0 against 22.2).
+// expert of 256 rows: 15.5 against 21.8 us) and lose from two on (512 rows: 27.0 against 22.2).  All of that at 4096 columns: with few,
+// the rule is up to 1.5 times off (128 experts of 24 rows x 256 x 512: 12.9 us, tiles of 128 x 256 8.7).
 template<typename Out>
 cudaError_t launch_product(const ProductArgs& a, int sm_count, cudaStream_t stream)
 {
