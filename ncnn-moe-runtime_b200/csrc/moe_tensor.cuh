@@ -8,7 +8,7 @@
 
 namespace moe {
 
-constexpr uint32_t kSpinLimit = 1u << 20; // looks at a barrier before a wait gives up: one that fails is held for 4 us, so 4 s
+constexpr uint32_t kSpinLimit = 1u << 18; // looks at a barrier before a wait gives up: one that fails is held for 4 us, so a second
 
 // ---- mbarriers, tensor memory, descriptors ---------------------------------------------
 
